@@ -22,6 +22,9 @@ enum DeviceError : int {
   DEV_TIMEOUT_PEER_FLAG = 0x401,
   DEV_BAD_TOKEN = 0x301,
   DEV_BAD_POSITION = 0x302,
+  DEV_BAD_BATCH = 0x303,  // a sequence's rows or length outside the call's sizes
+  DEV_BAD_PAGE = 0x304,   // a page id outside the pool
+  DEV_BAD_LOGITS = 0x305, // a row of logits without any token to draw
 };
 
 // A wait gives up after this many nanoseconds of polling (about 2 s: far

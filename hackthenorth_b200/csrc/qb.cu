@@ -1856,6 +1856,10 @@ static int read_device_error(int* err_word, cudaStream_t st, std::string* msg) {
   char buf[128];
   if (v == DEV_BAD_TOKEN) return set_err(msg, QB_ERR_ARG, "token id outside the vocabulary");
   if (v == DEV_BAD_POSITION) return set_err(msg, QB_ERR_CAPACITY, "position outside the KV capacity");
+  if (v == DEV_BAD_BATCH)
+    return set_err(msg, QB_ERR_ARG, "a sequence's query rows or cached length lie outside the call's sizes");
+  if (v == DEV_BAD_PAGE) return set_err(msg, QB_ERR_ARG, "a page id lies outside the pool");
+  if (v == DEV_BAD_LOGITS) return set_err(msg, QB_ERR_ARG, "a row of logits holds no token that can be drawn");
   std::snprintf(buf, sizeof(buf), "device wait timed out (site 0x%x); kernel returned early", v);
   return set_err(msg, QB_ERR_TIMEOUT, buf);
 }
@@ -2185,3 +2189,5 @@ extern "C" int qb_grouped_attention_noalloc(const void* q, const void* k_cache, 
   if (e != cudaSuccess) return cuda_fail(nullptr, e, "attention launch");
   return QB_OK;
 }
+
+#include "serving.cuh"

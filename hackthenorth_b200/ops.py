@@ -8,12 +8,15 @@ the CUDA library; there is no PyTorch or CPU fallback.
 """
 from __future__ import annotations
 
+import contextlib
+
 import torch
 
 from . import _lib
 
 BF16 = torch.bfloat16
 _scratch = {}
+_workspaces = {}
 
 
 def _op_scratch(device) -> torch.Tensor:
@@ -45,7 +48,11 @@ def _bf16_cuda(*ts):
 def check_device_errors(device=None) -> None:
     """Synchronise and raise if an op-level kernel reported a device error."""
     buf = _op_scratch(device or torch.cuda.current_device())
-    _lib.check(_lib.load().qb_op_check(buf.data_ptr(), _lib.stream_handle()))
+    try:
+        _lib.check(_lib.load().qb_op_check(buf.data_ptr(), _lib.stream_handle()))
+    except Exception:
+        _workspaces.clear()  # a kernel that gave up may have left its tickets mid-count
+        raise
 
 
 def norm_projection(x, gain, weight, eps=1e-6, *, swiglu=False):
@@ -166,3 +173,139 @@ def rope_attention(qkv, q_norm, k_norm, cos, sin, keys, values, position, eps=1e
                                              cap, position.data_ptr(), out.data_ptr(), scratch.data_ptr(),
                                              scratch.numel(), _lib.stream_handle()))
     return out
+
+
+# ------------------------------------------------------ paged K/V cache, sampling
+# These calls run on the device their tensors are on (current or not), on its
+# current stream, and may overlap on different streams: each stream has its own
+# workspace, and a call made while a graph is captured takes one from the
+# graph's own memory, so graphs share none either.
+
+def _status(device) -> int:
+    """Address of the device error word that ``check_device_errors`` reads."""
+    buf = _scratch.get(device.index)
+    if buf is None:
+        if torch.cuda.is_current_stream_capturing():
+            raise RuntimeError("call an operator once on this device before capturing a graph")
+        buf = _op_scratch(device)
+    return buf.data_ptr()
+
+
+def _workspace(device, stream: int, nbytes: int) -> torch.Tensor:
+    zero = 8192  # qb_paged_zero_bytes()
+    if torch.cuda.is_current_stream_capturing():
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf[:zero].zero_()
+        return buf
+    key = (device.index, stream)
+    buf = _workspaces.get(key)
+    if buf is None or buf.numel() < nbytes:
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
+        buf[:zero].zero_()
+        _workspaces[key] = buf
+    return buf
+
+
+def _on(device):
+    """Make ``device`` current for the call (the library launches there)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _batch(device, k_pages, v_pages, page_table, q_start, kv_lens):
+    """Checked (pages, Hkv, page, table width, sequences) of a paged batch."""
+    _require(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == 128,
+             "expected k_pages and v_pages [pages, Hkv, page, 128]")
+    for t in (k_pages, v_pages):
+        _require(t.dtype == BF16 and t.device == device and t.is_contiguous(),
+                 "expected contiguous bf16 pools on the device of the queries")
+    for t in (page_table, q_start, kv_lens):
+        _require(t.dtype == torch.int32 and t.device == device and t.is_contiguous(),
+                 "page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the queries")
+    _require(page_table.dim() == 2 and kv_lens.dim() == 1 and q_start.dim() == 1
+             and page_table.shape[0] == kv_lens.shape[0] and q_start.shape[0] == kv_lens.shape[0] + 1,
+             "expected page_table [B, P], q_start [B + 1], kv_lens [B]")
+    return (*k_pages.shape[:3], page_table.shape[1], kv_lens.shape[0])
+
+
+def _rows_out(out, shape, device):
+    if out is None:
+        return torch.empty(shape, dtype=BF16, device=device)
+    _require(out.dtype == BF16 and out.device == device and out.is_contiguous() and tuple(out.shape) == tuple(shape),
+             "out must be a contiguous bf16 tensor of the result's shape on the device of the queries")
+    return out
+
+
+def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_table, q_start, kv_lens, eps=1e-6,
+                      n_heads=None, first_position=0, out=None):
+    """Per-head q/k RMSNorm and RoPE of packed rows, K and V appended to a paged cache.
+
+    qkv ``[T, (Hq + 2 Hkv) 128]``; q_norm/k_norm ``[128]`` or None (no norm);
+    cos/sin ``[positions, 128]``; k_pages/v_pages ``[pages, Hkv, page, 128]``
+    written in place; page_table int32 ``[B, P]``, q_start int32 ``[B + 1]``,
+    kv_lens int32 ``[B]`` (keys of each sequence once its rows are appended)
+    -> rotated q ``[T, Hq, 128]``. Row i of sequence b, rows ``q_start[b]`` to
+    ``q_start[b + 1]``, goes to slot ``kv_lens[b] - n + i`` and is turned by
+    the angle of ``first_position`` more (the length of a shared prefix). Rows
+    from ``q_start[B]`` on are left as they are in ``out``. Page ids, lengths
+    or positions out of range are skipped and raise in ``check_device_errors``.
+    ``dryft/engine/kernels/fused.py:9-30,47-82`` for a ragged batch."""
+    _bf16_cuda(qkv, q_norm, k_norm, cos, sin)
+    dev = qkv.device
+    pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
+    _require(qkv.dim() == 2 and qkv.shape[1] % 128 == 0, "expected qkv [T, (Hq + 2 Hkv) 128]")
+    hq = n_heads if n_heads is not None else qkv.shape[1] // 128 - 2 * hkv
+    _require(hq > 0 and qkv.shape[1] == (hq + 2 * hkv) * 128, "packed qkv width does not match the cache heads")
+    _require(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == 128, "expected cos and sin [positions, 128]")
+    for t in (q_norm, k_norm, cos, sin):
+        _require(t is None or t.device == dev, "norms and rope tables must be on the device of qkv")
+    for t in (q_norm, k_norm):
+        _require(t is None or t.numel() == 128, "norm gains must have 128 entries")
+    tokens = qkv.shape[0]
+    with _on(dev):
+        out = _rows_out(out, (tokens, hq, 128), dev)
+        _lib.check(_lib.load().qb_rope_paged_append(
+            qkv.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), cos.data_ptr(), sin.data_ptr(), cos.shape[0], float(eps),
+            k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width, q_start.data_ptr(),
+            kv_lens.data_ptr(), seqs, tokens, int(first_position), hq, hkv, out.data_ptr(), _status(dev),
+            _lib.stream_handle()))
+    return out
+
+
+def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0, sinks=0, max_queries=None, out=None):
+    """Causal GQA attention of packed query rows over a paged cache.
+
+    q ``[T, Hq, 128]`` (normalised, rotated), the rest as in
+    ``rope_paged_append`` -> ``[T, Hq, 128]``. The query at position p sees
+    key c iff ``c <= p`` and (``window == 0`` or ``c > p - window`` or ``c <
+    sinks``). Pages without a key that some row sees are not read, so they may
+    have been given back (any id in the table). ``max_queries`` bounds the query
+    rows of a sequence (default T; a tight bound picks the faster kernel); a
+    longer sequence raises in ``check_device_errors``. Rows from ``q_start[B]``
+    on are left as they are in ``out``; a row that sees no key gives 0. A value
+    that is not finite in a key that one row of a sequence sees may reach that
+    sequence's other rows. ``dryft/engine/kernels/attention.py:200-237`` for a
+    ragged batch."""
+    _bf16_cuda(q)
+    dev = q.device
+    pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
+    _require(q.dim() == 3 and q.shape[2] == 128 and q.shape[1] % hkv == 0, "expected q [T, Hq, 128], Hq a multiple of Hkv")
+    tokens, hq = q.shape[:2]
+    if max_queries is None:
+        max_queries = tokens
+    L = _lib.load()
+    with _on(dev):
+        out = _rows_out(out, q.shape, dev)
+        need = _paged_bytes(dev, max_queries, hq, hkv)
+        stream = _lib.stream_handle()
+        ws = _workspace(dev, stream, need)
+        _lib.check(L.qb_paged_attention(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
+            q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, int(max_queries), hq, hkv, int(window), int(sinks),
+            out.data_ptr(), ws.data_ptr(), need, _status(dev), stream))
+    return out
+
+
+def _paged_bytes(device, max_queries, hq, hkv) -> int:
+    n = _lib.c_size_t()
+    _lib.check(_lib.load().qb_paged_workspace_bytes(max_queries, hq, hkv, _lib.ctypes.byref(n)))
+    return n.value

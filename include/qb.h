@@ -317,6 +317,66 @@ int qb_grouped_attention_noalloc(const void* q, const void* k_cache, const void*
                                  const int64_t* positions, void* out, int* device_status,
                                  void* stream);
 
+/* ---- operators over a paged K/V cache --------------------------------------
+ *
+ * The reference keeps one contiguous cache per sequence
+ * (dryft/engine/decode.py:25-46); these are its attention sublayer's calls for
+ * sequences that share one pool of pages.
+ *   k_pages, v_pages  [num_pages][Hkv][page_size][128] bf16; page_size 16, 32,
+ *                     64, 128 or 256
+ *   page_table        device int32 [n_seqs][table_width]: key c of sequence b
+ *                     is slot c % page_size of page page_table[b][c / page_size];
+ *                     entries that no visible key needs are not read
+ *   q_start           device int32 [n_seqs + 1], ascending from 0 or more:
+ *                     sequence b owns query rows q_start[b] .. q_start[b + 1] - 1
+ *                     (none is allowed); rows from q_start[n_seqs] on belong to
+ *                     no sequence: their outputs are left as they are
+ *   kv_lens           device int32 [n_seqs]: cached keys of the sequence, those
+ *                     of its query rows included; query i of n sits at position
+ *                     kv_lens[b] - n + i (a negative one sees nothing: output 0)
+ *   tokens            rows of q (and of out)
+ * At most 1024 sequences, 64 KV heads and 16 query heads per KV head. Lengths
+ * and tables are read on the device (a captured graph follows them); numbers
+ * outside the call's sizes are reported through device_status (a device int,
+ * zero before, for instance the first word of a qb_op_check scratch) and the
+ * sequence, page or row is skipped: the output of that sequence is then not
+ * defined. All pointers belong to the current device. */
+
+/* Per-head q/k RMSNorm (skipped when the gain is NULL), rotate-half RoPE and
+ * the append of K and V: the norm_rope_cache step
+ * (dryft/engine/kernels/fused.py:9-30,47-82) for any number of sequences.
+ * qkv [tokens][Hq*128 + 2*Hkv*128]; rope_cos/rope_sin [table_rows][128] bf16;
+ * row i of sequence b goes to slot p = kv_lens[b] - n + i of its pages and is
+ * turned by the angle of position first_position + p (first_position: keys of
+ * a shared prefix that precede every sequence's own). q_out [tokens][Hq][128].
+ * fp32 arithmetic, one rounding to bf16 at the end. A position below 0 or
+ * beyond the rope table is reported and skipped. Pages of different sequences
+ * must not overlap where rows are written. */
+int qb_rope_paged_append(const void* qkv, const void* q_norm, const void* k_norm, const void* rope_cos,
+                         const void* rope_sin, int table_rows, float eps, void* k_pages, void* v_pages, int num_pages,
+                         int page_size, const int* page_table, int table_width, const int* q_start,
+                         const int* kv_lens, int n_seqs, int tokens, int first_position, int n_heads, int n_kv_heads,
+                         void* q_out, int* device_status, void* stream);
+
+/* Workspace of qb_paged_attention; its first qb_paged_zero_bytes() bytes must
+ * be zero before its first use (the kernels leave them zero). Calls that may
+ * overlap on the GPU need a workspace each. */
+size_t qb_paged_zero_bytes(void);
+int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, size_t* bytes);
+
+/* Attention of packed query rows over their sequences' pages (the grouped
+ * attention of dryft/engine/kernels/attention.py:200-237 for a ragged batch).
+ * Query position p sees key c iff c <= p and (window == 0, or c > p - window,
+ * or c < sinks): window 0 is full causal attention, sinks the number of first
+ * keys that stay visible beside a window. Keys that no row sees are not read,
+ * their pages included. max_queries: an upper bound of every sequence's query
+ * rows (a longer sequence is reported and skipped). q, out [tokens][Hq][128]
+ * bf16, q normalised and rotated. */
+int qb_paged_attention(const void* q, const void* k_pages, const void* v_pages, int num_pages, int page_size,
+                       const int* page_table, int table_width, const int* q_start, const int* kv_lens, int n_seqs,
+                       int tokens, int max_queries, int n_heads, int n_kv_heads, int window, int sinks, void* out,
+                       void* workspace, size_t workspace_bytes, int* device_status, void* stream);
+
 /* Read the device error word of an op-level scratch (synchronises stream). */
 int qb_op_check(void* scratch, void* stream);
 
