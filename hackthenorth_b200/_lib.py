@@ -74,9 +74,11 @@ SIGNATURES = {
     "qb_rope_paged_append": (c_int, [c_void_p] * 5 + [c_int, c_float] + [c_void_p] * 2 + [c_int] * 2 + [c_void_p, c_int]
                              + [c_void_p] * 2 + [c_int] * 5 + [c_void_p] * 3),
     "qb_paged_zero_bytes": (c_size_t, []),
-    "qb_paged_workspace_bytes": (c_int, [c_int, c_int, c_int, ctypes.POINTER(c_size_t)]),
+    "qb_paged_workspace_bytes": (c_int, [c_int] * 4 + [ctypes.POINTER(c_size_t)]),
     "qb_paged_attention": (c_int, [c_void_p] * 3 + [c_int] * 2 + [c_void_p, c_int] + [c_void_p] * 2 + [c_int] * 7
                            + [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "qb_shared_prefix_attention": (c_int, [c_void_p] * 3 + [c_int] * 2 + [c_void_p, c_int, c_int, c_void_p, c_int]
+                                   + [c_void_p] * 2 + [c_int] * 5 + [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "qb_op_check": (c_int, [c_void_p, c_void_p]),
     "qb_grouped_attention_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                              c_void_p, c_void_p, c_void_p]),

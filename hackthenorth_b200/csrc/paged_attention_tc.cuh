@@ -1,0 +1,616 @@
+// paged_attention_tc.cuh — attention of many query rows over a paged cache on
+// the tcgen05 tensor cores: prompts, chunks of prompts, verify rows, mixed
+// batches, and the pass over a prefix that a whole batch shares.
+//
+// The formula and the masks are those of paged_decode.cuh. A unit is up to 256
+// query rows of one sequence (two M = 128 tiles of 128 / G tokens with the G
+// query heads of one KV head) against the 128-key tiles that some of its rows
+// sees. As there, the units' tiles form one line which is cut evenly over the
+// CTAs (one per SM); a cut unit leaves (m, l, O) of its pieces in the
+// workspace, and paged_join_kernel joins them: with 256 rows a piece is 128 KB,
+// too much for one CTA to join behind the others.
+//
+// Bound by the tensor cores where every key tile meets 256 rows (512 MMA-cycles
+// each for S and P.V of a tile and M tile) and by the cache's bytes below that.
+//  * warp 0: TMA. Q tiles (3D map, 128-byte swizzle) and K and V tiles of
+//    32 KB, a box per page, into two slots each.
+//  * warp 1, one lane: the MMAs. S_t = Q_t . K^T into TMEM columns 128 t, and
+//    once tile t's softmax has put P_t (bf16) over the first half of S_t,
+//    O_t += P_t . V with P_t read from TMEM into columns 256 + 128 t. S_t of the
+//    next key tile follows P_t . V in issue order, which is the order of
+//    execution, so one M tile's softmax runs under the other's MMAs.
+//  * warps 4-7 and 8-11: softmax of M tile 0 and 1, a thread per row. The
+//    reference maximum only moves when a row's maximum grows by more than 8 (P
+//    stays below 2^8 and keeps its relative precision), so O is seldom rescaled.
+// The register file is split by setmaxnreg: 384 threads start with 168 each
+// (64512); the first warpgroup keeps 56, the softmax groups take 224:
+// 128 * 56 + 256 * 224 = 64512.
+// Every wait is bounded; on failure an error is recorded, the roles stop, and
+// TMEM is released after the MMAs that were issued.
+#pragma once
+#include "paged_decode.cuh"
+#include "prefill_attention_tc.cuh"
+
+namespace qb {
+
+constexpr int kPtKeys = 128;
+constexpr int kPtRows = 256;
+constexpr int kPtThreads = 12 * 32;
+constexpr int kPtTile = 128 * 128 * 2;  // a Q, K or V tile: 32 KB, dims 0-63 then 64-127
+constexpr int kPtMaxUnits = 7168;
+constexpr int kPtMinTiles = 2;
+
+struct PtUnit {  // a cut unit, for the join
+  int token0, tokens, head, last, first_slot, valid;
+};
+
+struct PagedTcArgs {
+  PagedBatch b;
+  int Hq, Hkv, G, max_units;
+  RowSink sink;
+  float* part_o;   // [2 CTAs][256][128]
+  float* part_ml;  // [2 CTAs][256][2]
+  PtUnit* cut;     // [CTAs]
+  int* err;
+};
+
+__host__ inline size_t pt_smem_bytes(int max_units) {
+  return 1024 + 6 * (size_t)kPtTile + 256 + (size_t)(kPagedMaxSeqs + 1 + max_units + 1) * 4;
+}
+
+// d += A (TMEM) . B (shared memory)
+__device__ __forceinline__ void tc_mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
+      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      : "memory");
+}
+// 32 columns of this warp's lanes without the wait (tc_ld_wait follows).
+__device__ __forceinline__ void tc_ld32_async(uint32_t taddr, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tc_st32_async(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+      "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void tc_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+// The wait, and a use of the registers after it, so that no use moves above.
+template <int N>
+__device__ __forceinline__ void tc_ld_wait(uint32_t (&r)[N]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
+}
+
+// Unit u of the launch: its sequence, tokens and key tiles.
+struct TcUnit {
+  int seq, token0, tokens, p_first, kv, hi;  // p_first: position of token0; hi: one past the last key a row sees
+  TileSpan ts;
+};
+__device__ __forceinline__ TcUnit tc_unit(const PagedBatch& b, const int* seq_unit, int u, int per_unit) {
+  int lo = 0, hi = b.n_seqs - 1;
+  while (lo < hi) {  // the sequence of unit u: the first with seq_unit[seq + 1] > u
+    const int mid = (lo + hi) >> 1;
+    if (seq_unit[mid + 1] > u) hi = mid;
+    else lo = mid + 1;
+  }
+  const SeqSpan sp = paged_seq(b, lo, nullptr);
+  TcUnit r;
+  r.seq = lo;
+  const int i0 = (u - seq_unit[lo]) * per_unit;
+  r.token0 = sp.q0 + i0;
+  r.tokens = min(per_unit, sp.n - i0);
+  r.kv = sp.kv;
+  if (b.q_start == nullptr) {  // every row sees all keys
+    r.p_first = sp.kv - 1;
+    r.hi = sp.kv;
+  } else {
+    r.p_first = sp.kv - sp.n + i0;
+    r.hi = r.p_first + r.tokens;
+  }
+  r.ts = tile_span<kPtKeys>(r.p_first, r.hi, b.window, b.sinks);
+  return r;
+}
+
+// Inclusive sum of v over the block's threads on top of carry (updated).
+__device__ __forceinline__ int block_scan(int v, int* warp_tot, int& carry) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int u = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += u;
+  }
+  if (lane == 31) warp_tot[warp] = v;
+  __syncthreads();
+  int before = carry, all = 0;
+  for (int w = 0; w < (int)blockDim.x / 32; ++w) {
+    if (w < warp) before += warp_tot[w];
+    all += warp_tot[w];
+  }
+  carry += all;
+  __syncthreads();
+  return before + v;
+}
+
+__global__ void __launch_bounds__(kPtThreads, 1)
+    paged_tc_kernel(const __grid_constant__ CUtensorMap tmq, const __grid_constant__ CUtensorMap tmk,
+                    const __grid_constant__ CUtensorMap tmv, const PagedTcArgs a) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = qs + 2 * kPtTile;  // K, V, K, V
+  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + 4 * kPtTile);
+  uint64_t* kv_full = bars;        // [4]
+  uint64_t* kv_empty = bars + 4;   // [4]
+  uint64_t* q_full = bars + 8;     // [2]
+  uint64_t* q_empty = bars + 10;   // [2]
+  uint64_t* s_full = bars + 12;    // [2]
+  uint64_t* p_full = bars + 14;    // [2]
+  uint64_t* o_done = bars + 16;    // [2]
+  uint64_t* done = bars + 18;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  int* warp_tot = reinterpret_cast<int*>(tmem_slot + 2);  // [12]
+  int* seq_unit = reinterpret_cast<int*>(bars) + 64;      // [n_seqs + 1] units before each sequence
+  int* unit_tile = seq_unit + kPagedMaxSeqs + 1;          // [units + 1] tiles before each unit
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const PagedBatch& b = a.b;
+  const int RH = 128 / a.G;  // tokens per M tile
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < 4; ++s) {
+      mbar_init(&kv_full[s], 1);
+      mbar_init(&kv_empty[s], 1);
+    }
+    for (int t = 0; t < 2; ++t) {
+      mbar_init(&q_full[t], 1);
+      mbar_init(&q_empty[t], 1);
+      mbar_init(&s_full[t], 1);
+      mbar_init(&p_full[t], 4);
+      mbar_init(&o_done[t], 1);
+    }
+    mbar_init(done, 1);
+    fence_mbar_init();
+    flags[0] = 0;
+    seq_unit[0] = 0;
+    unit_tile[0] = 0;
+    prefetch_tensormap(&tmq);
+    prefetch_tensormap(&tmk);
+    prefetch_tensormap(&tmv);
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)),
+                 "r"(512)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+  pdl_wait();
+  pdl_trigger();
+
+  // ---- the line of tiles
+  int units = 0;
+  for (int s0 = 0; s0 < b.n_seqs; s0 += kPtThreads) {
+    const int s = s0 + threadIdx.x;
+    const int n = s < b.n_seqs ? paged_seq(b, s, a.err).n : 0;
+    const int v = block_scan((n + 2 * RH - 1) / (2 * RH), warp_tot, units);
+    if (s < b.n_seqs) seq_unit[s + 1] = v;
+  }
+  __syncthreads();
+  if (units > a.max_units) {  // sequences that overlap
+    if (threadIdx.x == 0) report_error(a.err, DEV_BAD_BATCH);
+    units = a.max_units;
+  }
+  int tiles = 0;
+  for (int u0 = 0; u0 < units; u0 += kPtThreads) {
+    const int u = u0 + threadIdx.x;
+    const int v = block_scan(u < units ? tc_unit(b, seq_unit, u, 2 * RH).ts.count : 0, warp_tot, tiles);
+    if (u < units) unit_tile[u + 1] = v;
+  }
+  __syncthreads();
+  const long long total = (long long)tiles * a.Hkv;
+  const int E = (int)min((long long)gridDim.x, max(1ll, total / kPtMinTiles));
+  const int me = blockIdx.x;
+  const bool busy = me < E && total > 0;
+  const long long t_begin = busy ? tile_begin(me, total, E) : 0, t_end = busy ? tile_begin(me + 1, total, E) : 0;
+  int unit0 = 0;
+  {
+    int lo = 0, hi = max(0, units - 1);
+    while (lo < hi) {  // the unit of tile t_begin
+      const int mid = (lo + hi) >> 1;
+      if ((long long)unit_tile[mid + 1] * a.Hkv > t_begin) hi = mid;
+      else lo = mid + 1;
+    }
+    unit0 = lo;
+  }
+  if (threadIdx.x == 0) a.cut[me].valid = 0;
+  __syncthreads();
+
+  // Every role walks the same pieces: f(unit, head, first tile, end tile, tiles of the unit, its place in the line).
+  auto walk = [&](auto&& f) {
+    long long t = t_begin;
+    for (int u = unit0; t < t_end; ++u) {
+      const TcUnit un = tc_unit(b, seq_unit, u, 2 * RH);
+      const int n = unit_tile[u + 1] - unit_tile[u];
+      const long long base = (long long)unit_tile[u] * a.Hkv;
+      const long long stop = min(t_end, base + (long long)n * a.Hkv);
+      while (t < stop) {
+        const int g = (int)((t - base) / n);
+        const long long u0 = base + (long long)g * n;
+        const int k0 = (int)(t - u0), k1 = (int)min((long long)n, k0 + (t_end - t));
+        if (!f(un, g, k0, k1, n, u0, t)) return;
+        t += k1 - k0;
+      }
+    }
+  };
+  auto tile_key = [&](const TileSpan& ts, int k) { return (k < ts.n_sink ? k : k - ts.n_sink + ts.lo_tile) * kPtKeys; };
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+      // -------------------------------------------------------------- producer
+      const int br = min(1 << b.page_log2, kPtKeys), nbox = kPtKeys / br;
+      const int kind = lane & 3, box = lane >> 2;
+      int issued = 0, quse[2] = {0, 0};
+      bool ok = true;
+      walk([&](const TcUnit& un, int g, int k0, int k1, int, long long, long long) {
+        auto page_of = [&](int k) {
+          const int c0 = tile_key(un.ts, k) + box * br;
+          if (k >= k1 || box >= nbox || c0 >= un.hi || !(b.window == 0 || c0 + br > un.ts.lo || c0 < b.sinks)) return -1;
+          const int page = b.page_table[(size_t)un.seq * b.table_width + (c0 >> b.page_log2)];
+          if (page < 0 || page >= b.num_pages) {
+            report_error(a.err, DEV_BAD_PAGE);
+            return -1;
+          }
+          return page;
+        };
+        int page = page_of(k0);
+        for (int t = 0; t < (un.tokens > RH ? 2 : 1) && ok; ++t) {
+          if (quse[t] > 0) ok = __all_sync(0xffffffffu, mbar_wait(&q_empty[t], (quse[t] - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY));
+          if (!ok) break;
+          ++quse[t];
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&q_full[t], (uint32_t)RH * a.G * 256);
+            for (int h = 0; h < 2; ++h)
+              tma_load_3d(qs + t * kPtTile + h * (kPtTile / 2), &tmq, 64 * h, g * a.G, un.token0 + t * RH, &q_full[t]);
+          }
+        }
+        for (int k = k0; k < k1 && ok; ++k) {
+          const int c0 = tile_key(un.ts, k) + box * br;
+          const int now = page;
+          page = page_of(k + 1);  // its load runs while the slots are waited for
+          const int y = ((now * a.Hkv + g) << b.page_log2) + (c0 & ((1 << b.page_log2) - 1));
+          const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, now >= 0 && kind < 2)) * br * 128;
+#pragma unroll
+          for (int kv = 0; kv < 2; ++kv) {
+            const int s = 2 * (issued & 1) + kv;
+            if (issued >= 2)
+              ok = ok && __all_sync(0xffffffffu, mbar_wait(&kv_empty[s], ((issued >> 1) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY));
+            if (!ok) break;
+            if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], bytes);
+            __syncwarp();
+            if (now >= 0 && (kind >> 1) == kv)
+              tma_load_2d(ring + s * kPtTile + (kind & 1) * (kPtTile / 2) + box * br * 128, kv ? &tmv : &tmk,
+                          64 * (kind & 1), y, &kv_full[s]);
+          }
+          if (ok) ++issued;
+        }
+        if (flags[0] != 0) ok = false;
+        return ok;
+      });
+      if (!ok) flags[0] = 1;
+      // keep shared memory alive until every issued copy has landed (after a failure a K tile may have no V: the
+      // waits are bounded)
+      for (int t = 0; t < 2; ++t)
+        if (quse[t] > 0) mbar_wait(&q_full[t], (quse[t] - 1) & 1, nullptr, 0);
+      for (int i = max(0, issued - 2); i < issued + (ok ? 0 : 1); ++i)
+        for (int kv = 0; kv < 2; ++kv) mbar_wait(&kv_full[2 * (i & 1) + kv], (i >> 1) & 1, nullptr, 0);
+    } else if (warp == 1 && lane == 0) {
+      // ------------------------------------------------------------ MMA issuer
+      const uint32_t idesc_s = pg_idesc(128, kPtKeys);
+      const uint32_t idesc_o = pg_idesc(128, 128) | (1u << 16);  // B (V) MN-major
+      int J = 0, quse[2] = {0, 0}, puse[2] = {0, 0};
+      bool ok = true;
+      walk([&](const TcUnit& un, int, int k0, int k1, int, long long, long long) {
+        const int nt = un.tokens > RH ? 2 : 1;
+        auto issue_s = [&](int t, int j) {  // S_t of key tile j of this CTA
+          const uint8_t* kt = ring + 2 * (j & 1) * kPtTile;
+#pragma unroll
+          for (int k = 0; k < 8; ++k) {
+            const uint64_t ad = ft_desc(qs + t * kPtTile + (k >> 2) * (kPtTile / 2), 16, 1024) + (uint64_t)((k & 3) * 2);
+            const uint64_t bd = ft_desc(kt + (k >> 2) * (kPtTile / 2), 16, 1024) + (uint64_t)((k & 3) * 2);
+            tc_mma(tmem + (uint32_t)(t * 128), ad, bd, idesc_s, k > 0 ? 1u : 0u);
+          }
+          tc_commit(&s_full[t]);
+        };
+        ok = ok && mbar_wait(&kv_full[2 * (J & 1)], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+        for (int t = 0; t < nt && ok; ++t) {
+          ok = mbar_wait(&q_full[t], quse[t] & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          if (!ok) break;
+          ++quse[t];
+          tc_fence_after();
+          issue_s(t, J);
+          if (k1 - k0 == 1) tc_commit(&q_empty[t]);
+        }
+        if (ok) tc_commit(&kv_empty[2 * (J & 1)]);
+        for (int k = k0; k < k1 && ok; ++k, ++J) {
+          const uint8_t* vt = ring + (2 * (J & 1) + 1) * kPtTile;
+          ok = mbar_wait(&kv_full[2 * (J & 1) + 1], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          for (int t = 0; t < nt && ok; ++t) {
+            ok = mbar_wait(&p_full[t], puse[t] & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
+            if (!ok) break;
+            ++puse[t];
+            tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)  // 16 keys a step
+              tc_mma_ta(tmem + (uint32_t)(256 + 128 * t), tmem + (uint32_t)(128 * t + 8 * ks),
+                        ft_desc(vt + ks * 2048, kPtTile / 2, 1024), idesc_o, (k > k0 || ks > 0) ? 1u : 0u);
+            tc_commit(&o_done[t]);
+            if (t == nt - 1) tc_commit(&kv_empty[2 * (J & 1) + 1]);
+            if (k + 1 < k1) {
+              if (t == 0) ok = mbar_wait(&kv_full[2 * ((J + 1) & 1)], ((J + 1) >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+              if (!ok) break;
+              tc_fence_after();
+              issue_s(t, J + 1);
+              if (k + 2 == k1) tc_commit(&q_empty[t]);
+              if (t == nt - 1) tc_commit(&kv_empty[2 * ((J + 1) & 1)]);
+            }
+          }
+        }
+        return ok;
+      });
+      if (!ok) flags[0] = 1;
+      tc_commit(done);  // TMEM is released below only after every MMA issued here has completed
+      mbar_wait(done, 0, nullptr, 0);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    // ----------------------------------------------------------------- softmax
+    const int t = (warp - 4) >> 2;  // M tile
+    const int qrow = (warp & 3) * 32 + lane;
+    const int qi = qrow / a.G, hj = qrow - qi * a.G;
+    const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
+    const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + 256 + 128 * t;
+    const float scale = kLog2e * 0.08838834764831845f;  // log2(e) / sqrt(128)
+    int J = 0, suse = 0;
+    walk([&](const TcUnit& un, int g, int k0, int k1, int n, long long u0, long long at) {
+      if (t * RH >= un.tokens) {
+        J += k1 - k0;
+        return true;
+      }
+      const int token = t * RH + qi;  // of the unit
+      const bool valid = qi < RH && token < un.tokens;
+      const int pos = !valid ? -1 : b.q_start == nullptr ? un.kv - 1 : un.p_first + token;
+      float m_ref = -INFINITY, l = 0.f;
+      for (int k = k0; k < k1; ++k, ++J, ++suse) {
+        const int c0 = tile_key(un.ts, k);
+        bool ok = mbar_wait(&s_full[t], suse & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
+        if (!__all_sync(0xffffffffu, ok)) return false;
+        tc_fence_after();
+        uint32_t sr[128];
+#pragma unroll
+        for (int c = 0; c < 4; ++c) tc_ld32_async(s_col + 32 * c, sr + 32 * c);
+        tc_ld_wait(sr);
+        // keys [lo, hi) and [0, first) of the tile are visible to this row
+        const int hi = pos - c0 + 1;
+        const int lo = b.window > 0 ? pos - b.window + 1 - c0 : 0;
+        const int first = b.sinks - c0;
+        if (!__all_sync(0xffffffffu, hi >= kPtKeys && (lo <= 0 || first >= kPtKeys))) {
+#pragma unroll
+          for (int c = 0; c < 128; ++c)
+            if (!(c < hi && (c >= lo || c < first))) sr[c] = 0xff800000u;  // -inf, whatever the score was
+        }
+        float mx[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) mx[e] = __uint_as_float(sr[e]);
+#pragma unroll
+        for (int c = 8; c < 128; ++c) mx[c & 7] = fmaxf(mx[c & 7], __uint_as_float(sr[c]));
+        const float m_new = scale * fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
+                                          fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+        // A row that has seen nothing has O = l = 0: its reference moves freely.
+        if (m_ref == -INFINITY) m_ref = m_new;
+        if (__any_sync(0xffffffffu, m_new > m_ref + 8.f)) {
+          ok = mbar_wait(&o_done[t], (suse - 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          if (!__all_sync(0xffffffffu, ok)) return false;
+          tc_fence_after();
+          const float top = fmaxf(m_ref, m_new);
+          const float corr = m_ref == -INFINITY ? 1.f : exp2f(m_ref - top);
+#pragma unroll 1
+          for (int c = 0; c < 128; c += 8) {
+            float ov[8];
+            tc_ld8(o_col + c, ov);
+            asm volatile(
+                "tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(o_col + c),
+                "r"(__float_as_uint(ov[0] * corr)), "r"(__float_as_uint(ov[1] * corr)),
+                "r"(__float_as_uint(ov[2] * corr)), "r"(__float_as_uint(ov[3] * corr)),
+                "r"(__float_as_uint(ov[4] * corr)), "r"(__float_as_uint(ov[5] * corr)),
+                "r"(__float_as_uint(ov[6] * corr)), "r"(__float_as_uint(ov[7] * corr))
+                : "memory");
+          }
+          tc_st_wait();
+          l *= corr;
+          m_ref = top;
+        }
+        const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < 128; c += 4) {  // P over S's own registers: two bf16 a register
+          float p[4];
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            p[e] = ex2_approx(fmaf(__uint_as_float(sr[c + e]), scale, -mu));
+            rs[e] += p[e];
+          }
+          sr[c >> 1] = pack_bf16(p[0], p[1]);
+          sr[(c >> 1) + 1] = pack_bf16(p[2], p[3]);
+        }
+        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        tc_st32_async(s_col, sr);
+        tc_st32_async(s_col + 32, sr + 32);
+        tc_st_wait();
+        if (c0 + kPtKeys > un.hi || (b.window > 0 && c0 < un.ts.lo && c0 + kPtKeys > b.sinks)) {
+          // V rows that no row of the unit sees may hold anything: their P is 0, but 0 * NaN is NaN
+          ok = mbar_wait(&kv_full[2 * (J & 1) + 1], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          if (!__all_sync(0xffffffffu, ok)) return false;
+          const int c = c0 + qrow;
+          if (c >= un.hi || (b.window > 0 && c < un.ts.lo && c >= b.sinks)) {
+            uint8_t* vr = ring + (2 * (J & 1) + 1) * kPtTile + qrow * 128;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+              *reinterpret_cast<uint4*>(vr + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(vr + kPtTile / 2 + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+            }
+          }
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[t]);
+      }
+      // ---- the piece's rows
+      bool ok = mbar_wait(&o_done[t], (suse - 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+      if (!__all_sync(0xffffffffu, ok)) return false;
+      tc_fence_after();
+      const bool whole = k0 == 0 && k1 == n;
+      const int slot = 2 * me + (at == t_begin ? 0 : 1);
+      const size_t row = (size_t)(un.token0 + token) * a.Hq + g * a.G + hj;
+      const bool has_base = a.sink.base32 != nullptr;
+      RowScale rs = {1.f, 0.f, 0.f};
+      if (whole && valid) rs = row_scale(m_ref, l, has_base, has_base ? a.sink.base_lse[row] : 0.f);
+#pragma unroll 1
+      for (int c = 0; c < 4; ++c) {
+        float ov[32];
+        tc_ld32(o_col + 32 * c, ov);
+        if (!valid) continue;
+#pragma unroll
+        for (int e = 0; e < 32; ++e) ov[e] *= rs.own;
+        if (!whole || a.sink.out32 != nullptr) {
+          float* dst = whole ? a.sink.out32 + row * kAttnD + 32 * c
+                             : a.part_o + ((size_t)slot * kPtRows + t * 128 + qrow) * kAttnD + 32 * c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4*>(dst + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+        } else {
+          if (has_base) {
+            const float* bv = a.sink.base32 + row * kAttnD + 32 * c;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              const float4 x = *reinterpret_cast<const float4*>(bv + e);
+              ov[e] = fmaf(x.x, rs.other, ov[e]);
+              ov[e + 1] = fmaf(x.y, rs.other, ov[e + 1]);
+              ov[e + 2] = fmaf(x.z, rs.other, ov[e + 2]);
+              ov[e + 3] = fmaf(x.w, rs.other, ov[e + 3]);
+            }
+          }
+          bf16* dst = a.sink.out + row * kAttnD + 32 * c;
+#pragma unroll
+          for (int e = 0; e < 32; e += 8)
+            *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack_bf16(ov[e], ov[e + 1]), pack_bf16(ov[e + 2], ov[e + 3]),
+                                                            pack_bf16(ov[e + 4], ov[e + 5]), pack_bf16(ov[e + 6], ov[e + 7]));
+        }
+      }
+      if (valid) {
+        if (!whole) {
+          float* ml = a.part_ml + ((size_t)slot * kPtRows + t * 128 + qrow) * 2;
+          ml[0] = m_ref;
+          ml[1] = l;
+        } else if (a.sink.lse32 != nullptr) {
+          a.sink.lse32[row] = rs.lse;
+        }
+      }
+      if (!whole && k0 == 0 && t == 0 && qrow == 0) {
+        PtUnit* c = &a.cut[me];
+        c->token0 = un.token0;
+        c->tokens = un.tokens;
+        c->head = g;
+        c->last = tile_owner(u0 + n - 1, total, E);
+        c->first_slot = at == t_begin ? 0 : 1;
+        c->valid = 1;
+      }
+      tc_fence_before();  // O_t is read before the next unit's MMAs write it (through p_full)
+      return true;
+    });
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512) : "memory");
+  }
+}
+
+// Joins the pieces of the units that paged_tc_kernel cut: blockIdx.x is the
+// CTA whose last piece begins the unit, blockIdx.y takes 32 of its rows, a
+// warp a row at a time, a lane 4 dims. Bytes: the pieces once (L2).
+constexpr int kPjRows = 32;
+constexpr int kPjThreads = 256;
+__global__ void __launch_bounds__(kPjThreads) paged_join_kernel(const PagedTcArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const PtUnit un = a.cut[blockIdx.x];
+  if (!un.valid) return;
+  const int RH = 128 / a.G, first = blockIdx.x;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool has_base = a.sink.base32 != nullptr;
+  for (int i = warp; i < kPjRows; i += kPjThreads / 32) {
+    const int r = blockIdx.y * kPjRows + i, t = r >> 7, qrow = r & 127;
+    const int qi = qrow / a.G, token = t * RH + qi;
+    if (qi >= RH || token >= un.tokens) continue;
+    auto piece = [&](int c) { return (size_t)(2 * c + (c == first ? un.first_slot : 0)) * kPtRows + r; };
+    float top = -INFINITY;
+    for (int c = first + lane; c <= un.last; c += 32) top = fmaxf(top, a.part_ml[piece(c) * 2]);
+    top = warp_max(top);
+    const float mu = top == -INFINITY ? 0.f : top;
+    float lsum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int c = first; c <= un.last; ++c) {
+      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + piece(c) * 2);
+      const float4 ov = *reinterpret_cast<const float4*>(a.part_o + piece(c) * kAttnD + 4 * lane);
+      const float w = exp2f(ml.x - mu);
+      lsum = fmaf(ml.y, w, lsum);
+      acc.x = fmaf(ov.x, w, acc.x);
+      acc.y = fmaf(ov.y, w, acc.y);
+      acc.z = fmaf(ov.z, w, acc.z);
+      acc.w = fmaf(ov.w, w, acc.w);
+    }
+    const size_t row = (size_t)(un.token0 + token) * a.Hq + un.head * a.G + qrow % a.G;
+    const RowScale rs = row_scale(top, lsum, has_base, has_base ? a.sink.base_lse[row] : 0.f);
+    acc.x *= rs.own; acc.y *= rs.own; acc.z *= rs.own; acc.w *= rs.own;
+    if (has_base) {
+      const float4 bv = *reinterpret_cast<const float4*>(a.sink.base32 + row * kAttnD + 4 * lane);
+      acc.x = fmaf(bv.x, rs.other, acc.x);
+      acc.y = fmaf(bv.y, rs.other, acc.y);
+      acc.z = fmaf(bv.z, rs.other, acc.z);
+      acc.w = fmaf(bv.w, rs.other, acc.w);
+    }
+    if (a.sink.out32 != nullptr) {
+      *reinterpret_cast<float4*>(a.sink.out32 + row * kAttnD + 4 * lane) = acc;
+      if (lane == 0 && a.sink.lse32 != nullptr) a.sink.lse32[row] = rs.lse;
+    } else {
+      uint2 ob;
+      ob.x = pack_bf16(acc.x, acc.y);
+      ob.y = pack_bf16(acc.z, acc.w);
+      *reinterpret_cast<uint2*>(a.sink.out + row * kAttnD + 4 * lane) = ob;
+    }
+  }
+}
+
+}  // namespace qb

@@ -2,21 +2,13 @@
 // tensor maps, workspace layout and launches. Included at the end of qb.cu
 // (it uses that file's error, launch and tensor-map helpers).
 #pragma once
+#include "paged_attention_tc.cuh"
 #include "paged_decode.cuh"
 
 namespace {
 
 constexpr size_t kPagedZeroBytes = 8192;  // tickets: the workspace's part that must start at zero
 constexpr int kPagedMaxCtas = (int)(kPagedZeroBytes / 4);
-
-struct PagedPools {
-  CUtensorMap k, v;
-};
-
-// Boxes of min(page, 64) rows x 64 dims over the pool as rows of 128 dims.
-bool make_pool_map(CUtensorMap* m, const void* base, long long rows, int box_rows) {
-  return make_rows_map(m, base, rows, kAttnD, box_rows);
-}
 
 int check_pages(int num_pages, int page_size, int n_kv_heads, int table_width, int n_seqs, int tokens) {
   if (page_size < 16 || page_size > 256 || (page_size & (page_size - 1)) != 0)
@@ -45,36 +37,188 @@ int log2_of(int v) {
 }
 
 // Workspace: tickets (zero-filled by the caller once, left at zero), then the
-// pieces' (m, l) and O.
-struct DecodeWorkspace {
-  int grid;
-  size_t ml, o, bytes;
+// cut units, the pieces' (m, l) and O of the kernel that runs, and for a shared
+// prefix every row's result over the prefix.
+struct PagedWorkspace {
+  size_t cut, ml, o, base_lse, base, bytes;
 };
-DecodeWorkspace decode_workspace(int sms) {
-  DecodeWorkspace w;
-  w.grid = std::min(sms * kPdCtasPerSm, kPagedMaxCtas);
-  w.ml = kPagedZeroBytes;
-  w.o = w.ml + align_up((size_t)2 * w.grid * kPdRows * 2 * sizeof(float), 256);
-  w.bytes = w.o + (size_t)2 * w.grid * kPdRows * kAttnD * sizeof(float);
+PagedWorkspace paged_workspace(int grid, int rows, long long base_rows) {
+  PagedWorkspace w;
+  w.cut = kPagedZeroBytes;
+  w.ml = w.cut + align_up((size_t)grid * sizeof(PtUnit), 256);
+  w.o = w.ml + align_up((size_t)2 * grid * rows * 2 * sizeof(float), 256);
+  w.base_lse = w.o + (size_t)2 * grid * rows * kAttnD * sizeof(float);
+  w.base = w.base_lse + align_up((size_t)base_rows * sizeof(float), 256);
+  w.bytes = w.base + (size_t)base_rows * kAttnD * sizeof(float);
   return w;
+}
+int decode_grid() { return std::min(current_sm_count() * kPdCtasPerSm, kPagedMaxCtas); }
+int tc_grid() { return std::min(current_sm_count(), kPagedMaxCtas); }
+
+// Whether the few-rows kernel takes the call: its 16 MMA rows hold every
+// sequence's query rows of a KV head.
+bool few_rows(int max_queries, int G) { return (long long)max_queries * G <= kPdRows; }
+
+PagedWorkspace workspace_for(int max_queries, int G, int n_heads, int prefix_tokens) {
+  const bool tc = !few_rows(max_queries, G) || prefix_tokens > 0;
+  // the few-rows kernel's pieces fit in the other's room, which a prefix's second pass uses
+  static_assert(kPdCtasPerSm * kPdRows <= kPtRows, "pieces of the few-rows kernel");
+  return tc ? paged_workspace(tc_grid(), kPtRows, (long long)prefix_tokens * n_heads)
+            : paged_workspace(decode_grid(), kPdRows, 0);
+}
+
+// One device's function attribute, set once.
+template <typename K>
+cudaError_t smem_attr(K kernel, bool (&set)[kMaxDevices], size_t bytes) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess || (dev < kMaxDevices && set[dev])) return e;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+  if (e == cudaSuccess && dev < kMaxDevices) set[dev] = true;
+  return e;
 }
 
 cudaError_t launch_paged_decode(const CUtensorMap& k, const CUtensorMap& v, PagedAttnArgs a, uint8_t* ws,
-                                cudaStream_t st) {
-  static bool attr[kMaxDevices] = {};
-  int dev = 0;
-  cudaError_t e = cudaGetDevice(&dev);
+                                const PagedWorkspace& w, cudaStream_t st) {
+  static bool set[kMaxDevices] = {};
+  cudaError_t e = smem_attr(paged_decode_kernel, set, pd_smem_bytes());
   if (e != cudaSuccess) return e;
-  if (dev >= kMaxDevices || !attr[dev]) {
-    e = cudaFuncSetAttribute(paged_decode_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)pd_smem_bytes());
-    if (e != cudaSuccess) return e;
-    if (dev < kMaxDevices) attr[dev] = true;
-  }
-  const DecodeWorkspace w = decode_workspace(current_sm_count());
   a.tickets = reinterpret_cast<unsigned*>(ws);
   a.part_ml = reinterpret_cast<float*>(ws + w.ml);
   a.part_o = reinterpret_cast<float*>(ws + w.o);
-  return launch_ex(paged_decode_kernel, dim3(w.grid), dim3(kPdThreads), pd_smem_bytes(), st, k, v, a);
+  return launch_ex(paged_decode_kernel, dim3(decode_grid()), dim3(kPdThreads), pd_smem_bytes(), st, k, v, a);
+}
+
+// Units of a launch: full ones, and one begun by each sequence.
+long long tc_units(int tokens, int n_seqs, int G) { return tokens / (2 * (128 / G)) + std::min(n_seqs, tokens); }
+
+cudaError_t launch_paged_tc(const CUtensorMap& q, const CUtensorMap& k, const CUtensorMap& v, PagedTcArgs a,
+                            uint8_t* ws, const PagedWorkspace& w, cudaStream_t st) {
+  static bool set[kMaxDevices] = {};
+  cudaError_t e = smem_attr(paged_tc_kernel, set, pt_smem_bytes(kPtMaxUnits));
+  if (e != cudaSuccess) return e;
+  a.cut = reinterpret_cast<PtUnit*>(ws + w.cut);
+  a.part_ml = reinterpret_cast<float*>(ws + w.ml);
+  a.part_o = reinterpret_cast<float*>(ws + w.o);
+  const int grid = tc_grid();
+  e = launch_ex(paged_tc_kernel, dim3(grid), dim3(kPtThreads), pt_smem_bytes(a.max_units), st, q, k, v, a);
+  if (e != cudaSuccess) return e;
+  return launch_ex(paged_join_kernel, dim3(grid, kPtRows / kPjRows), dim3(kPjThreads), 0, st, a);
+}
+
+int check_tiles(int tokens, int n_seqs, int G, int table_width, int page_size) {
+  const long long units = tc_units(tokens, n_seqs, G);
+  if (units > kPtMaxUnits) return set_err(nullptr, QB_ERR_UNSUPPORTED, "more than 7168 blocks of 256 query rows per KV head");
+  if (std::max((long long)n_seqs, units) * ((long long)table_width * page_size / kPdKeys + 2) > 0x7fffffffll)
+    return set_err(nullptr, QB_ERR_UNSUPPORTED, "more than 2^31 key tiles over all sequences");
+  return QB_OK;
+}
+
+// Attention of the whole call; prefix_len 0: without a shared prefix.
+int run_paged_attention(const void* q, const void* k_pages, const void* v_pages, int num_pages, int page_size,
+                        const int* prefix_table, int prefix_pages, int prefix_len, const int* page_table,
+                        int table_width, const int* q_start, const int* kv_lens, int n_seqs, int tokens,
+                        int max_queries, int n_heads, int n_kv_heads, int window, int sinks, void* out,
+                        void* workspace, size_t workspace_bytes, int* device_status, void* stream) {
+  if (!ptr_ok(k_pages) || !ptr_ok(v_pages) || !ptr_ok(workspace))
+    return set_err(nullptr, QB_ERR_ARG, "pools and workspace must be 16-byte aligned device pointers");
+  if (!page_table || !q_start || !kv_lens || !device_status)
+    return set_err(nullptr, QB_ERR_ARG, "page_table, q_start, kv_lens and device_status must be device pointers");
+  int rc = check_heads(n_heads, n_kv_heads);
+  if (rc == QB_OK) rc = check_pages(num_pages, page_size, n_kv_heads, table_width, n_seqs, tokens);
+  if (rc != QB_OK) return rc;
+  const int G = n_heads / n_kv_heads;
+  if (window < 0 || sinks < 0) return set_err(nullptr, QB_ERR_ARG, "window and sinks must not be negative");
+  if (prefix_len < 0 || prefix_pages < 0 || (long long)prefix_len > (long long)prefix_pages * page_size)
+    return set_err(nullptr, QB_ERR_ARG, "prefix_len must lie in 0..prefix_pages x page_size");
+  if (prefix_len > 0 && !prefix_table) return set_err(nullptr, QB_ERR_ARG, "prefix_table must be a device pointer");
+  if (max_queries < 1 && tokens > 0) return set_err(nullptr, QB_ERR_ARG, "max_queries must be at least 1");
+  if (tokens == 0) return QB_OK;
+  if (!ptr_ok(q) || !ptr_ok(out)) return set_err(nullptr, QB_ERR_ARG, "q and out must be 16-byte aligned device pointers");
+  if (max_queries > tokens) max_queries = tokens;
+  rc = check_tiles(tokens, n_seqs, G, table_width, page_size);
+  if (rc == QB_OK && prefix_len > 0) {
+    rc = check_pages(num_pages, page_size, n_kv_heads, prefix_pages, 1, tokens);
+    if (rc == QB_OK) rc = check_tiles(tokens, 1, G, prefix_pages, page_size);
+  }
+  if (rc != QB_OK) return rc;
+  const bool few = few_rows(max_queries, G);
+  const PagedWorkspace w = workspace_for(max_queries, G, n_heads, prefix_len > 0 ? tokens : 0);
+  if (workspace_bytes < w.bytes) return set_err(nullptr, QB_ERR_ARG, "workspace smaller than qb_paged_workspace_bytes()");
+  uint8_t* ws = static_cast<uint8_t*>(workspace);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+
+  PagedBatch b;
+  std::memset(&b, 0, sizeof(b));
+  b.page_table = page_table;
+  b.q_start = q_start;
+  b.kv_lens = kv_lens;
+  b.n_seqs = n_seqs;
+  b.tokens = tokens;
+  b.table_width = table_width;
+  b.num_pages = num_pages;
+  b.page_log2 = log2_of(page_size);
+  b.max_queries = max_queries;
+  b.window = std::min(window, 1 << 30);  // longer than any sequence: the whole of it
+  b.sinks = std::min(sinks, 1 << 30);
+  RowSink sink;
+  std::memset(&sink, 0, sizeof(sink));
+  sink.out = static_cast<bf16*>(out);
+
+  const long long rows = (long long)num_pages * n_kv_heads * page_size;
+  CUtensorMap mq, mk, mv;
+  if (!few || prefix_len > 0) {
+    const int box = std::min(page_size, kPtKeys);
+    if (!make_q3_map(&mq, q, tokens, n_heads, G, 128 / G) || !make_rows_map(&mk, k_pages, rows, kAttnD, box) ||
+        !make_rows_map(&mv, v_pages, rows, kAttnD, box))
+      return set_err(nullptr, QB_ERR_CUDA, "cuTensorMapEncodeTiled failed for q or the page pools");
+    PagedTcArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.Hq = n_heads;
+    a.Hkv = n_kv_heads;
+    a.G = G;
+    a.err = device_status;
+    if (prefix_len > 0) {  // the prefix once for all rows, as one sequence whose rows see every key
+      a.b = b;
+      a.b.page_table = prefix_table;
+      a.b.q_start = nullptr;
+      a.b.kv_lens = nullptr;
+      a.b.n_seqs = 1;
+      a.b.table_width = prefix_pages;
+      a.b.kv_all = prefix_len;
+      a.b.window = a.b.sinks = 0;
+      a.max_units = (int)tc_units(tokens, 1, G);
+      a.sink.out32 = reinterpret_cast<float*>(ws + w.base);
+      a.sink.lse32 = reinterpret_cast<float*>(ws + w.base_lse);
+      cudaError_t e = launch_paged_tc(mq, mk, mv, a, ws, w, st);
+      if (e != cudaSuccess) return cuda_fail(nullptr, e, "shared prefix launch");
+      sink.base32 = a.sink.out32;
+      sink.base_lse = a.sink.lse32;
+    }
+    if (!few) {
+      a.b = b;
+      a.max_units = (int)tc_units(tokens, n_seqs, G);
+      a.sink = sink;
+      cudaError_t e = launch_paged_tc(mq, mk, mv, a, ws, w, st);
+      if (e != cudaSuccess) return cuda_fail(nullptr, e, "paged attention launch");
+      return QB_OK;
+    }
+  }
+  const int box = std::min(page_size, kPdKeys);
+  if (!make_rows_map(&mk, k_pages, rows, kAttnD, box) || !make_rows_map(&mv, v_pages, rows, kAttnD, box))
+    return set_err(nullptr, QB_ERR_CUDA, "cuTensorMapEncodeTiled failed for the page pools");
+  PagedAttnArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.b = b;
+  a.q = static_cast<const bf16*>(q);
+  a.Hq = n_heads;
+  a.Hkv = n_kv_heads;
+  a.G = G;
+  a.sink = sink;
+  a.err = device_status;
+  cudaError_t e = launch_paged_decode(mk, mv, a, ws, w, st);
+  if (e != cudaSuccess) return cuda_fail(nullptr, e, "paged attention launch");
+  return QB_OK;
 }
 
 }  // namespace
@@ -129,12 +273,12 @@ int qb_rope_paged_append(const void* qkv, const void* q_norm, const void* k_norm
   return QB_OK;
 }
 
-int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, size_t* bytes) {
+int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, int prefix_tokens, size_t* bytes) {
   if (!bytes) return set_err(nullptr, QB_ERR_ARG, "bytes is NULL");
+  if (prefix_tokens < 0 || prefix_tokens > (1 << 24)) return set_err(nullptr, QB_ERR_UNSUPPORTED, "0..2^24 query rows");
   int rc = check_heads(n_heads, n_kv_heads);
   if (rc != QB_OK) return rc;
-  (void)max_queries;
-  *bytes = decode_workspace(current_sm_count()).bytes;
+  *bytes = workspace_for(max_queries, n_heads / n_kv_heads, n_heads, prefix_tokens).bytes;
   return QB_OK;
 }
 
@@ -142,51 +286,19 @@ int qb_paged_attention(const void* q, const void* k_pages, const void* v_pages, 
                        const int* page_table, int table_width, const int* q_start, const int* kv_lens, int n_seqs,
                        int tokens, int max_queries, int n_heads, int n_kv_heads, int window, int sinks, void* out,
                        void* workspace, size_t workspace_bytes, int* device_status, void* stream) {
-  if (!ptr_ok(k_pages) || !ptr_ok(v_pages) || !ptr_ok(workspace))
-    return set_err(nullptr, QB_ERR_ARG, "pools and workspace must be 16-byte aligned device pointers");
-  if (!page_table || !q_start || !kv_lens || !device_status)
-    return set_err(nullptr, QB_ERR_ARG, "page_table, q_start, kv_lens and device_status must be device pointers");
-  int rc = check_heads(n_heads, n_kv_heads);
-  if (rc == QB_OK) rc = check_pages(num_pages, page_size, n_kv_heads, table_width, n_seqs, tokens);
-  if (rc != QB_OK) return rc;
-  if (window < 0 || sinks < 0) return set_err(nullptr, QB_ERR_ARG, "window and sinks must not be negative");
-  if (max_queries < 1 && tokens > 0) return set_err(nullptr, QB_ERR_ARG, "max_queries must be at least 1");
-  if (tokens == 0) return QB_OK;
-  if (!ptr_ok(q) || !ptr_ok(out)) return set_err(nullptr, QB_ERR_ARG, "q and out must be 16-byte aligned device pointers");
-  const int G = n_heads / n_kv_heads;
-  if (max_queries > tokens) max_queries = tokens;
-  size_t need = 0;
-  rc = qb_paged_workspace_bytes(max_queries, n_heads, n_kv_heads, &need);
-  if (rc != QB_OK) return rc;
-  if (workspace_bytes < need) return set_err(nullptr, QB_ERR_ARG, "workspace smaller than qb_paged_workspace_bytes()");
-  PagedAttnArgs a;
-  std::memset(&a, 0, sizeof(a));
-  a.b.page_table = page_table;
-  a.b.q_start = q_start;
-  a.b.kv_lens = kv_lens;
-  a.b.n_seqs = n_seqs;
-  a.b.tokens = tokens;
-  a.b.table_width = table_width;
-  a.b.num_pages = num_pages;
-  a.b.page_log2 = log2_of(page_size);
-  a.b.max_queries = max_queries;
-  a.b.window = std::min(window, 1 << 30);  // longer than any sequence: the whole of it
-  a.b.sinks = std::min(sinks, 1 << 30);
-  a.q = static_cast<const bf16*>(q);
-  a.Hq = n_heads;
-  a.Hkv = n_kv_heads;
-  a.G = G;
-  a.sink.out = static_cast<bf16*>(out);
-  a.err = device_status;
-  CUtensorMap mk, mv;
-  const long long rows = (long long)num_pages * n_kv_heads * page_size;
-  const int box = std::min(page_size, kPdKeys);
-  if (!make_pool_map(&mk, k_pages, rows, box) || !make_pool_map(&mv, v_pages, rows, box))
-    return set_err(nullptr, QB_ERR_CUDA, "cuTensorMapEncodeTiled failed for the page pools");
-  if (max_queries * G > kPdRows) return set_err(nullptr, QB_ERR_UNSUPPORTED, "more than 16 query rows per KV head");
-  cudaError_t e = launch_paged_decode(mk, mv, a, static_cast<uint8_t*>(workspace), static_cast<cudaStream_t>(stream));
-  if (e != cudaSuccess) return cuda_fail(nullptr, e, "paged attention launch");
-  return QB_OK;
+  return run_paged_attention(q, k_pages, v_pages, num_pages, page_size, nullptr, 0, 0, page_table, table_width, q_start,
+                             kv_lens, n_seqs, tokens, max_queries, n_heads, n_kv_heads, window, sinks, out, workspace,
+                             workspace_bytes, device_status, stream);
+}
+
+int qb_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, int num_pages, int page_size,
+                               const int* prefix_table, int prefix_pages, int prefix_len, const int* page_table,
+                               int table_width, const int* q_start, const int* kv_lens, int n_seqs, int tokens,
+                               int max_queries, int n_heads, int n_kv_heads, void* out, void* workspace,
+                               size_t workspace_bytes, int* device_status, void* stream) {
+  return run_paged_attention(q, k_pages, v_pages, num_pages, page_size, prefix_table, prefix_pages, prefix_len,
+                             page_table, table_width, q_start, kv_lens, n_seqs, tokens, max_queries, n_heads, n_kv_heads,
+                             0, 0, out, workspace, workspace_bytes, device_status, stream);
 }
 
 }  // extern "C"

@@ -292,20 +292,49 @@ def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0,
     tokens, hq = q.shape[:2]
     if max_queries is None:
         max_queries = tokens
-    L = _lib.load()
     with _on(dev):
         out = _rows_out(out, q.shape, dev)
-        need = _paged_bytes(dev, max_queries, hq, hkv)
+        need = _paged_bytes(max_queries, hq, hkv, 0)
         stream = _lib.stream_handle()
         ws = _workspace(dev, stream, need)
-        _lib.check(L.qb_paged_attention(
+        _lib.check(_lib.load().qb_paged_attention(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
             q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, int(max_queries), hq, hkv, int(window), int(sinks),
             out.data_ptr(), ws.data_ptr(), need, _status(dev), stream))
     return out
 
 
-def _paged_bytes(device, max_queries, hq, hkv) -> int:
+def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_table, q_start, kv_lens,
+                            max_queries=None, out=None):
+    """``paged_attention`` (without a window) of a batch whose sequences all
+    begin with the same ``prefix_len`` keys, held once in the pages
+    ``prefix_table`` (int32 ``[n]``): one pass over them serves every sequence.
+    Each query sees the whole prefix and its sequence's own keys up to its
+    position; ``kv_lens`` and ``page_table`` count and place the own keys only
+    (append them with ``first_position=prefix_len``)."""
+    _bf16_cuda(q)
+    dev = q.device
+    pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
+    _require(q.dim() == 3 and q.shape[2] == 128 and q.shape[1] % hkv == 0, "expected q [T, Hq, 128], Hq a multiple of Hkv")
+    _require(prefix_table.dim() == 1 and prefix_table.dtype == torch.int32 and prefix_table.device == dev
+             and prefix_table.is_contiguous(), "prefix_table must be a contiguous int32 tensor [n] on the device of q")
+    tokens, hq = q.shape[:2]
+    if max_queries is None:
+        max_queries = tokens
+    with _on(dev):
+        out = _rows_out(out, q.shape, dev)
+        need = _paged_bytes(max_queries, hq, hkv, tokens)
+        stream = _lib.stream_handle()
+        ws = _workspace(dev, stream, need)
+        _lib.check(_lib.load().qb_shared_prefix_attention(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, prefix_table.data_ptr(),
+            prefix_table.shape[0], int(prefix_len), page_table.data_ptr(), width, q_start.data_ptr(),
+            kv_lens.data_ptr(), seqs, tokens, int(max_queries), hq, hkv, out.data_ptr(), ws.data_ptr(), need,
+            _status(dev), stream))
+    return out
+
+
+def _paged_bytes(max_queries, hq, hkv, prefix_tokens) -> int:
     n = _lib.c_size_t()
-    _lib.check(_lib.load().qb_paged_workspace_bytes(max_queries, hq, hkv, _lib.ctypes.byref(n)))
+    _lib.check(_lib.load().qb_paged_workspace_bytes(max_queries, hq, hkv, prefix_tokens, _lib.ctypes.byref(n)))
     return n.value

@@ -358,11 +358,13 @@ int qb_rope_paged_append(const void* qkv, const void* q_norm, const void* k_norm
                          const int* kv_lens, int n_seqs, int tokens, int first_position, int n_heads, int n_kv_heads,
                          void* q_out, int* device_status, void* stream);
 
-/* Workspace of qb_paged_attention; its first qb_paged_zero_bytes() bytes must
- * be zero before its first use (the kernels leave them zero). Calls that may
- * overlap on the GPU need a workspace each. */
+/* Workspace of qb_paged_attention (prefix_tokens 0) and
+ * qb_shared_prefix_attention (prefix_tokens: its `tokens`) for calls of up to
+ * max_queries; its first qb_paged_zero_bytes() bytes must be zero before its
+ * first use (the kernels leave them zero). Calls that may overlap on the GPU
+ * need a workspace each. */
 size_t qb_paged_zero_bytes(void);
-int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, size_t* bytes);
+int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, int prefix_tokens, size_t* bytes);
 
 /* Attention of packed query rows over their sequences' pages (the grouped
  * attention of dryft/engine/kernels/attention.py:200-237 for a ragged batch).
@@ -376,6 +378,19 @@ int qb_paged_attention(const void* q, const void* k_pages, const void* v_pages, 
                        const int* page_table, int table_width, const int* q_start, const int* kv_lens, int n_seqs,
                        int tokens, int max_queries, int n_heads, int n_kv_heads, int window, int sinks, void* out,
                        void* workspace, size_t workspace_bytes, int* device_status, void* stream);
+
+/* The same for a batch whose sequences all begin with the same prefix_len
+ * keys, kept once in prefix_table's pages (device int32 [prefix_pages]): they
+ * are attended to in one pass for the whole batch and joined with each
+ * sequence's own pages by the log-sum-exp. Every query sees the whole prefix,
+ * and of its own keys those at or below its position (full causal attention);
+ * kv_lens and page_table count and place the own keys only. prefix_len 0 is
+ * qb_paged_attention without a window. */
+int qb_shared_prefix_attention(const void* q, const void* k_pages, const void* v_pages, int num_pages, int page_size,
+                               const int* prefix_table, int prefix_pages, int prefix_len, const int* page_table,
+                               int table_width, const int* q_start, const int* kv_lens, int n_seqs, int tokens,
+                               int max_queries, int n_heads, int n_kv_heads, void* out, void* workspace,
+                               size_t workspace_bytes, int* device_status, void* stream);
 
 /* Read the device error word of an op-level scratch (synchronises stream). */
 int qb_op_check(void* scratch, void* stream);

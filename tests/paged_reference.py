@@ -48,6 +48,9 @@ def attention64(bt, window=0, sinks=0):
         if n == 0:
             continue
         a = bt["starts"][b]
+        if kv + prefix == 0:
+            out[a:a + n] = mag[a:a + n] = 0.0
+            continue
         p = torch.arange(kv - n, kv, device=out.device)[:, None]
         c = torch.arange(kv, device=out.device)[None]
         seen = c <= p

@@ -46,10 +46,32 @@ def test_attention_refuses(built_lib, kw, code):
     assert built_lib.qb_last_error(None)
 
 
+def _prefix(lib, **kw):
+    a = dict(q=PTR, k=PTR, v=PTR, pages=4, page=16, ptable=PTR, ppages=2, plen=20, table=PTR, width=4, q_start=PTR,
+             kv=PTR, seqs=1, tokens=1, max_q=1, hq=16, hkv=8, out=PTR, ws=PTR, ws_bytes=1 << 40, status=PTR, stream=None)
+    assert set(kw) <= set(a)
+    a.update(kw)
+    return lib.qb_shared_prefix_attention(*a.values())
+
+
+@pytest.mark.parametrize("kw,code", COMMON + [(dict(q=None), ARG), (dict(plen=-1), ARG), (dict(plen=33), ARG),
+                                              (dict(ptable=None), ARG), (dict(ppages=-1), ARG), (dict(max_q=0), ARG),
+                                              (dict(ws=None), ARG), (dict(ws_bytes=100), ARG)])
+def test_shared_prefix_refuses(built_lib, kw, code):
+    assert _prefix(built_lib, **kw) == code
+    assert built_lib.qb_last_error(None)
+
+
+def test_sizes_beyond_the_tile_counts_are_refused(built_lib):
+    assert _attention(built_lib, tokens=1 << 24, max_q=1 << 24, hq=128) == UNSUPPORTED  # too many blocks of rows
+    assert _attention(built_lib, seqs=1024, width=1 << 26) == UNSUPPORTED  # too many key tiles
+
+
 def test_empty_calls_return_without_a_launch(built_lib):
     assert _append(built_lib, tokens=0, qkv=None, out=None) == 0
     assert _attention(built_lib, tokens=0, q=None, out=None) == 0
     assert _attention(built_lib, tokens=0, max_q=0) == 0
+    assert _prefix(built_lib, tokens=0, q=None) == 0
 
 
 def test_python_calls_refuse_cpu_tensors():

@@ -146,3 +146,86 @@ def test_few_rows_match_formula(lens, hq, hkv, page, window, sinks):
     out = _attend(bt, **kw)
     _check(bt, out, window, sinks)
     assert torch.equal(out, _attend(bt, **kw))  # joins in a fixed order, tickets back at zero
+
+
+MANY = [
+    ([(17, 17)], 16, 8, 16),
+    ([(5, 9000)], 32, 8, 64),
+    ([(64, 64)], 32, 8, 64),
+    ([(65, 300), (1, 1), (0, 40), (129, 129), (1, 700), (33, 2049)], 32, 8, 32),
+    ([(17, 6000)], 4, 1, 128),
+    ([(700, 700)], 8, 4, 16),
+    ([(300, 1000), (7, 100)], 5, 1, 256),
+    ([(100, 100), (3, 200)], 16, 1, 16),
+    ([(260, 400)], 4, 4, 64),
+    ([(1 + i % 9, 20 + 37 * i % 400) for i in range(300)], 8, 8, 16),
+]
+
+
+@pytest.mark.parametrize("lens,hq,hkv,page", MANY)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (50, 4), (128, 128), (1000, 130)])
+def test_many_rows_match_formula(lens, hq, hkv, page, window, sinks):
+    bt = make_batch(lens, hq, hkv, page, 5, DEV, pad=3, scale=1.5)
+    _poison(bt, window, sinks)
+    kw = dict(window=window, sinks=sinks, max_queries=max(max(n for n, _ in lens), 17))
+    out = _attend(bt, **kw)
+    _check(bt, out, window, sinks)
+    assert torch.equal(out, _attend(bt, **kw))
+
+
+def test_rows_before_the_first_key_give_zero():
+    # more queries than cached keys: the first rows sit at negative positions and see nothing
+    for n, kv, hq in ((3, 1, 8), (2, 0, 8), (40, 9, 32)):
+        bt = make_batch([(n, kv), (1, 70)], hq, 8, 16, 11, DEV)
+        out = _attend(bt, max_queries=n)
+        assert bool((out[:n - kv] == 0).all())
+        _check(bt, out)
+
+
+def test_growing_scores_move_the_reference_maximum():
+    """Keys whose scores grow along the sequence: every tile lifts the running
+    maximum, the largest by far the last."""
+    for lens in ([(1, 700)], [(40, 700)]):
+        bt = make_batch(lens, 8, 8, 64, 13, DEV)
+        direction = torch.randn(D, generator=torch.Generator().manual_seed(1)).to(DEV)
+        bt["q"] = (direction.to(BF16).expand_as(bt["q"])).contiguous()
+        for c in range(700):
+            bt["k"][int(bt["pages"][0, c // 64]), :, c % 64] = (direction * (c / 700.0) ** 2 * 3).to(BF16)
+        ref, mag = attention64(bt)
+        out = _attend(bt, max_queries=lens[0][0])
+        # scores reach 40: a score's fp32 error is below 128 * 2^-24 * 40 = 2^-11.6, and so is its weight's
+        assert bool(((out.double() - ref).abs() <= attention_bound(ref, mag) + 2.0 ** -11 * mag).all())
+
+
+PREFIX = [
+    ([(1, 1)], 16, 8, 16, 1),
+    ([(1, 5), (1, 90), (1, 1)], 4, 1, 16, 1000),
+    ([(1, 1 + 7 * i) for i in range(40)], 32, 8, 64, 3001),
+    ([(4, 4), (1, 40), (0, 3), (2, 130)], 8, 4, 32, 129),
+    ([(9, 30), (40, 300), (1, 2)], 32, 8, 16, 777),
+    ([(30, 30)] * 9, 5, 1, 128, 256),
+    ([(1, 9), (2, 20)], 16, 8, 16, 0),
+]
+
+
+@pytest.mark.parametrize("lens,hq,hkv,page,prefix", PREFIX)
+def test_shared_prefix_matches_formula(lens, hq, hkv, page, prefix):
+    from hackthenorth_b200 import ops
+
+    bt = make_batch(lens, hq, hkv, page, 17, DEV, pad=2, scale=1.5, prefix=prefix)
+    own = torch.zeros(bt["k"].shape[0], page, dtype=torch.bool)
+    for ids, kv in [(bt["pages"][b].tolist(), kv if n else 0) for b, (n, kv) in enumerate(lens)] + [
+            (bt["prefix_table"].tolist(), prefix)]:
+        for c in range(kv):
+            own[ids[c // page], c % page] = True
+    for pool in (bt["k"], bt["v"]):
+        pool.masked_fill_(~own.to(DEV)[:, None, :, None], float("nan"))
+    outs = []
+    for _ in range(2):
+        out = torch.full_like(bt["q"], 7.0)
+        ops.shared_prefix_attention(bt["q"], bt["k"], bt["v"], bt["prefix_table"], prefix, bt["table"], bt["q_start"],
+                                    bt["kv_lens"], max_queries=max(n for n, _ in lens), out=out)
+        ops.check_device_errors(DEV)
+        _check(bt, out)
+        outs.append(out)
+    assert torch.equal(*outs)
