@@ -22,9 +22,13 @@
 //  * warps 4-7 and 8-11: softmax of M tile 0 and 1, a thread per row. The
 //    reference maximum only moves when a row's maximum grows by more than 8 (P
 //    stays below 2^8 and keeps its relative precision), so O is seldom rescaled.
+//  * warp 2, one lane: walks the CTA's pieces of units ahead of the others and
+//    hands them over through a ring of 4 (the lookups and divisions of a new
+//    piece took 3 us of every role's time when each made them itself).
 // The register file is split by setmaxnreg: 384 threads start with 168 each
-// (64512); the first warpgroup keeps 56, the softmax groups take 224:
-// 128 * 56 + 256 * 224 = 64512.
+// (64512); the first warpgroup keeps 104 (fewer spill: its roles' spills go to L2, as
+// shared memory leaves next to no L1), the softmax groups take 200:
+// 128 * 104 + 256 * 200 = 64512.
 // Every wait is bounded; on failure an error is recorded, the roles stop, and
 // TMEM is released after the MMAs that were issued.
 #pragma once
@@ -39,6 +43,19 @@ constexpr int kPtThreads = 12 * 32;
 constexpr int kPtTile = 128 * 128 * 2;  // a Q, K or V tile: 32 KB, dims 0-63 then 64-127
 constexpr int kPtMaxUnits = 7168;
 constexpr int kPtMinTiles = 2;
+
+constexpr int kPtPieces = 4;
+
+// What a CTA does next: the key tiles [k0, k1) of a unit (a role's whole state).
+struct PtPiece {
+  int seq, token0, tokens, p_first, hi, lo_tile, n_sink, lo;
+  int head, k0, k1;
+  int whole;  // the unit in one piece
+  int first;  // the CTA's first piece: its workspace slot is the first
+  int last;   // of a cut unit's first piece: the CTA of the last one; else -1
+  int pad[2];
+};
+static_assert(sizeof(PtPiece) == 64, "read as four 16-byte words");
 
 struct PtUnit {  // a cut unit, for the join
   int token0, tokens, head, last, first_slot, valid;
@@ -55,7 +72,7 @@ struct PagedTcArgs {
 };
 
 __host__ inline size_t pt_smem_bytes(int max_units) {
-  return 1024 + 6 * (size_t)kPtTile + 256 + (size_t)(kPagedMaxSeqs + 1 + max_units + 1) * 4;
+  return 1024 + 6 * (size_t)kPtTile + 512 + kPtPieces * sizeof(PtPiece) + (size_t)(kPagedMaxSeqs + 1 + max_units + 1) * 4;
 }
 
 // d += A (TMEM) . B (shared memory)
@@ -96,6 +113,16 @@ __device__ __forceinline__ void tc_ld_wait(uint32_t (&r)[N]) {
 #pragma unroll
   for (int i = 0; i < N; ++i) asm volatile("" : "+r"(r[i]));
 }
+
+// 32 bytes to a 32-byte aligned address in one store.
+__device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+               "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+               : "memory");
+}
+
+// A word with its lowest n bits set (n clamped to 0..32).
+__device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
 // Unit u of the launch: its sequence, tokens and key tiles.
 struct TcUnit {
@@ -159,13 +186,17 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   uint64_t* q_full = bars + 8;     // [2]
   uint64_t* q_empty = bars + 10;   // [2]
   uint64_t* s_full = bars + 12;    // [2]
-  uint64_t* p_full = bars + 14;    // [2]
-  uint64_t* o_done = bars + 16;    // [2]
-  uint64_t* done = bars + 18;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 19);
+  uint64_t* p_half = bars + 14;    // [2] P of the tile's keys 0-63
+  uint64_t* p_full = bars + 16;    // [2] P of all of them
+  uint64_t* o_done = bars + 18;    // [2]
+  uint64_t* piece_full = bars + 20;   // [4]
+  uint64_t* piece_empty = bars + 24;  // [4]
+  uint64_t* done = bars + 28;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* warp_tot = reinterpret_cast<int*>(tmem_slot + 2);  // [12]
-  int* seq_unit = reinterpret_cast<int*>(bars) + 64;      // [n_seqs + 1] units before each sequence
+  PtPiece* pieces = reinterpret_cast<PtPiece*>(bars + 64);
+  int* seq_unit = reinterpret_cast<int*>(pieces + kPtPieces);  // [n_seqs + 1] units before each sequence
   int* unit_tile = seq_unit + kPagedMaxSeqs + 1;          // [units + 1] tiles before each unit
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
@@ -180,10 +211,15 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
       mbar_init(&s_full[t], 1);
+      mbar_init(&p_half[t], 4);
       mbar_init(&p_full[t], 4);
       mbar_init(&o_done[t], 1);
     }
     mbar_init(done, 1);
+    for (int i = 0; i < kPtPieces; ++i) {
+      mbar_init(&piece_full[i], 1);
+      mbar_init(&piece_empty[i], 10);  // producer, MMA issuer, 8 softmax warps
+    }
     fence_mbar_init();
     flags[0] = 0;
     seq_unit[0] = 0;
@@ -230,50 +266,40 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   const int me = blockIdx.x;
   const bool busy = me < E && total > 0;
   const long long t_begin = busy ? tile_begin(me, total, E) : 0, t_end = busy ? tile_begin(me + 1, total, E) : 0;
-  int unit0 = 0;
-  {
-    int lo = 0, hi = max(0, units - 1);
-    while (lo < hi) {  // the unit of tile t_begin
-      const int mid = (lo + hi) >> 1;
-      if ((long long)unit_tile[mid + 1] * a.Hkv > t_begin) hi = mid;
-      else lo = mid + 1;
-    }
-    unit0 = lo;
-  }
   if (threadIdx.x == 0) a.cut[me].valid = 0;
   __syncthreads();
 
-  // Every role walks the same pieces: f(unit, head, first tile, end tile, tiles of the unit, its place in the line).
-  auto walk = [&](auto&& f) {
-    long long t = t_begin;
-    for (int u = unit0; t < t_end; ++u) {
-      const TcUnit un = tc_unit(b, seq_unit, u, 2 * RH);
-      const int n = unit_tile[u + 1] - unit_tile[u];
-      const long long base = (long long)unit_tile[u] * a.Hkv;
-      const long long stop = min(t_end, base + (long long)n * a.Hkv);
-      while (t < stop) {
-        const int g = (int)((t - base) / n);
-        const long long u0 = base + (long long)g * n;
-        const int k0 = (int)(t - u0), k1 = (int)min((long long)n, k0 + (t_end - t));
-        if (!f(un, g, k0, k1, n, u0, t)) return;
-        t += k1 - k0;
-      }
+  // Every role takes the same pieces in turn: f(piece), until an empty one. Lane 0 frees the entry.
+  auto walk = [&](uint32_t lanes_of_role, auto&& f) {
+    for (int i = 0;; ++i) {
+      const int e = i % kPtPieces;
+      if (!mbar_wait(&piece_full[e], (i / kPtPieces) & 1, a.err, DEV_TIMEOUT_ATTN_FULL)) return;
+      union {
+        uint4 w[4];
+        PtPiece p;
+      } u;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) u.w[j] = reinterpret_cast<const uint4*>(&pieces[e])[j];
+      __syncwarp(lanes_of_role);
+      if (lane == 0) mbar_arrive(&piece_empty[e]);
+      if (u.p.k0 == u.p.k1 || !f(u.p)) return;
     }
   };
-  auto tile_key = [&](const TileSpan& ts, int k) { return (k < ts.n_sink ? k : k - ts.n_sink + ts.lo_tile) * kPtKeys; };
+  auto tile_key = [&](const PtPiece& p, int k) { return (k < p.n_sink ? k : k - p.n_sink + p.lo_tile) * kPtKeys; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0) {
       // -------------------------------------------------------------- producer
       const int br = min(1 << b.page_log2, kPtKeys), nbox = kPtKeys / br;
       const int kind = lane & 3, box = lane >> 2;
       int issued = 0, quse[2] = {0, 0};
       bool ok = true;
-      walk([&](const TcUnit& un, int g, int k0, int k1, int, long long, long long) {
+      walk(0xffffffffu, [&](const PtPiece& un) {
+        const int g = un.head, k0 = un.k0, k1 = un.k1;
         auto page_of = [&](int k) {
-          const int c0 = tile_key(un.ts, k) + box * br;
-          if (k >= k1 || box >= nbox || c0 >= un.hi || !(b.window == 0 || c0 + br > un.ts.lo || c0 < b.sinks)) return -1;
+          const int c0 = tile_key(un, k) + box * br;
+          if (k >= k1 || box >= nbox || c0 >= un.hi || !(b.window == 0 || c0 + br > un.lo || c0 < b.sinks)) return -1;
           const int page = b.page_table[(size_t)un.seq * b.table_width + (c0 >> b.page_log2)];
           if (page < 0 || page >= b.num_pages) {
             report_error(a.err, DEV_BAD_PAGE);
@@ -293,7 +319,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
         }
         for (int k = k0; k < k1 && ok; ++k) {
-          const int c0 = tile_key(un.ts, k) + box * br;
+          const int c0 = tile_key(un, k) + box * br;
           const int now = page;
           page = page_of(k + 1);  // its load runs while the slots are waited for
           const int y = ((now * a.Hkv + g) << b.page_log2) + (c0 & ((1 << b.page_log2) - 1));
@@ -322,22 +348,71 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (quse[t] > 0) mbar_wait(&q_full[t], (quse[t] - 1) & 1, nullptr, 0);
       for (int i = max(0, issued - 2); i < issued + (ok ? 0 : 1); ++i)
         for (int kv = 0; kv < 2; ++kv) mbar_wait(&kv_full[2 * (i & 1) + kv], (i >> 1) & 1, nullptr, 0);
+    } else if (warp == 2 && lane == 0) {
+      // ------------------------------------------------------------- scheduler
+      int u = 0;
+      for (int hi = max(0, units - 1); u < hi;) {  // the unit of tile t_begin
+        const int mid = (u + hi) >> 1;
+        if ((long long)unit_tile[mid + 1] * a.Hkv > t_begin) hi = mid;
+        else u = mid + 1;
+      }
+      long long t = t_begin;
+      TcUnit un;
+      int n = 0, fresh = -1;  // fresh: the unit `un` describes
+      long long base = 0;
+      for (int i = 0;; ++i) {
+        const int e = i % kPtPieces;
+        PtPiece p;
+        p.k0 = p.k1 = 0;  // the end of the CTA's work
+        if (t < t_end) {
+          if (fresh != u) {
+            un = tc_unit(b, seq_unit, u, 2 * RH);
+            n = unit_tile[u + 1] - unit_tile[u];
+            base = (long long)unit_tile[u] * a.Hkv;
+            fresh = u;
+          }
+          const int g = (int)((t - base) / n);
+          const long long u0 = base + (long long)g * n;
+          p.seq = un.seq;
+          p.token0 = un.token0;
+          p.tokens = un.tokens;
+          p.p_first = un.p_first;
+          p.hi = un.hi;
+          p.lo_tile = un.ts.lo_tile;
+          p.n_sink = un.ts.n_sink;
+          p.lo = un.ts.lo;
+          p.head = g;
+          p.k0 = (int)(t - u0);
+          p.k1 = (int)min((long long)n, p.k0 + (t_end - t));
+          p.whole = p.k0 == 0 && p.k1 == n;
+          p.first = t == t_begin;
+          p.last = p.k0 == 0 && !p.whole ? tile_owner(u0 + n - 1, total, E) : -1;
+          t += p.k1 - p.k0;
+          if (g == a.Hkv - 1 && p.k1 == n) ++u;
+        }
+        if (i >= kPtPieces && !mbar_wait(&piece_empty[e], ((i / kPtPieces) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY)) break;
+        pieces[e] = p;
+        mbar_arrive(&piece_full[e]);
+        if (p.k0 == p.k1 || flags[0] != 0) break;
+      }
     } else if (warp == 1 && lane == 0) {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t idesc_s = pg_idesc(128, kPtKeys);
       const uint32_t idesc_o = pg_idesc(128, 128) | (1u << 16);  // B (V) MN-major
+      // descriptors made once; an offset of x bytes adds x >> 4 (the addresses stay below 2^18)
+      const uint64_t qd = ft_desc(qs, 16, 1024), kd = ft_desc(ring, 16, 1024);
+      const uint64_t vd = ft_desc(ring + kPtTile, kPtTile / 2, 1024);
       int J = 0, quse[2] = {0, 0}, puse[2] = {0, 0};
       bool ok = true;
-      walk([&](const TcUnit& un, int, int k0, int k1, int, long long, long long) {
+      walk(1u, [&](const PtPiece& un) {
+        const int k0 = un.k0, k1 = un.k1;
         const int nt = un.tokens > RH ? 2 : 1;
         auto issue_s = [&](int t, int j) {  // S_t of key tile j of this CTA
-          const uint8_t* kt = ring + 2 * (j & 1) * kPtTile;
+          const uint64_t qt = qd + (uint64_t)(t * (kPtTile >> 4)), kt = kd + (uint64_t)((j & 1) * (2 * kPtTile >> 4));
 #pragma unroll
-          for (int k = 0; k < 8; ++k) {
-            const uint64_t ad = ft_desc(qs + t * kPtTile + (k >> 2) * (kPtTile / 2), 16, 1024) + (uint64_t)((k & 3) * 2);
-            const uint64_t bd = ft_desc(kt + (k >> 2) * (kPtTile / 2), 16, 1024) + (uint64_t)((k & 3) * 2);
-            tc_mma(tmem + (uint32_t)(t * 128), ad, bd, idesc_s, k > 0 ? 1u : 0u);
-          }
+          for (int k = 0; k < 8; ++k)  // 16 dims a step
+            tc_mma(tmem + (uint32_t)(t * 128), qt + (k >> 2) * (kPtTile >> 5) + (k & 3) * 2,
+                   kt + (k >> 2) * (kPtTile >> 5) + (k & 3) * 2, idesc_s, k > 0 ? 1u : 0u);
           tc_commit(&s_full[t]);
         };
         ok = ok && mbar_wait(&kv_full[2 * (J & 1)], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
@@ -351,17 +426,22 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (ok) tc_commit(&kv_empty[2 * (J & 1)]);
         for (int k = k0; k < k1 && ok; ++k, ++J) {
-          const uint8_t* vt = ring + (2 * (J & 1) + 1) * kPtTile;
+          const uint64_t vt = vd + (uint64_t)((J & 1) * (2 * kPtTile >> 4));
           ok = mbar_wait(&kv_full[2 * (J & 1) + 1], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
           for (int t = 0; t < nt && ok; ++t) {
+            const uint32_t od = tmem + (uint32_t)(256 + 128 * t), pd = tmem + (uint32_t)(128 * t);
+            ok = mbar_wait(&p_half[t], puse[t] & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll
+            for (int ks = 0; ks < 4; ++ks)  // 16 keys a step
+              tc_mma_ta(od, pd + 8 * ks, vt + ks * 128, idesc_o, (k > k0 || ks > 0) ? 1u : 0u);
             ok = mbar_wait(&p_full[t], puse[t] & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
             if (!ok) break;
             ++puse[t];
             tc_fence_after();
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks)  // 16 keys a step
-              tc_mma_ta(tmem + (uint32_t)(256 + 128 * t), tmem + (uint32_t)(128 * t + 8 * ks),
-                        ft_desc(vt + ks * 2048, kPtTile / 2, 1024), idesc_o, (k > k0 || ks > 0) ? 1u : 0u);
+            for (int ks = 4; ks < 8; ++ks) tc_mma_ta(od, pd + 8 * ks, vt + ks * 128, idesc_o, 1u);
             tc_commit(&o_done[t]);
             if (t == nt - 1) tc_commit(&kv_empty[2 * (J & 1) + 1]);
             if (k + 1 < k1) {
@@ -381,7 +461,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_wait(done, 0, nullptr, 0);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ----------------------------------------------------------------- softmax
     const int t = (warp - 4) >> 2;  // M tile
     const int qrow = (warp & 3) * 32 + lane;
@@ -390,17 +470,18 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + 256 + 128 * t;
     const float scale = kLog2e * 0.08838834764831845f;  // log2(e) / sqrt(128)
     int J = 0, suse = 0;
-    walk([&](const TcUnit& un, int g, int k0, int k1, int n, long long u0, long long at) {
+    walk(0xffffffffu, [&](const PtPiece& un) {
+      const int k0 = un.k0, k1 = un.k1;
       if (t * RH >= un.tokens) {
         J += k1 - k0;
         return true;
       }
       const int token = t * RH + qi;  // of the unit
       const bool valid = qi < RH && token < un.tokens;
-      const int pos = !valid ? -1 : b.q_start == nullptr ? un.kv - 1 : un.p_first + token;
+      const int pos = !valid ? -1 : b.q_start == nullptr ? un.hi - 1 : un.p_first + token;
       float m_ref = -INFINITY, l = 0.f;
       for (int k = k0; k < k1; ++k, ++J, ++suse) {
-        const int c0 = tile_key(un.ts, k);
+        const int c0 = tile_key(un, k);
         bool ok = mbar_wait(&s_full[t], suse & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
         if (!__all_sync(0xffffffffu, ok)) return false;
         tc_fence_after();
@@ -414,8 +495,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int first = b.sinks - c0;
         if (!__all_sync(0xffffffffu, hi >= kPtKeys && (lo <= 0 || first >= kPtKeys))) {
 #pragma unroll
-          for (int c = 0; c < 128; ++c)
-            if (!(c < hi && (c >= lo || c < first))) sr[c] = 0xff800000u;  // -inf, whatever the score was
+          for (int w = 0; w < 4; ++w) {  // one bit a key, so that each score costs a test and a select
+            const uint32_t seen = bits_below(hi - 32 * w) & (~bits_below(lo - 32 * w) | bits_below(first - 32 * w));
+#pragma unroll
+            for (int c = 0; c < 32; ++c)  // -inf where unseen, whatever the score was
+              sr[32 * w + c] = (seen >> c) & 1u ? sr[32 * w + c] : 0xff800000u;
+          }
         }
         float mx[8];
 #pragma unroll
@@ -448,49 +533,54 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           l *= corr;
           m_ref = top;
         }
-        const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-        float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < 128; c += 4) {  // P over S's own registers: two bf16 a register
-          float p[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            p[e] = ex2_approx(fmaf(__uint_as_float(sr[c + e]), scale, -mu));
-            rs[e] += p[e];
-          }
-          sr[c >> 1] = pack_bf16(p[0], p[1]);
-          sr[(c >> 1) + 1] = pack_bf16(p[2], p[3]);
-        }
-        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
-        tc_st32_async(s_col, sr);
-        tc_st32_async(s_col + 32, sr + 32);
-        tc_st_wait();
-        if (c0 + kPtKeys > un.hi || (b.window > 0 && c0 < un.ts.lo && c0 + kPtKeys > b.sinks)) {
-          // V rows that no row of the unit sees may hold anything: their P is 0, but 0 * NaN is NaN
+        if (c0 + kPtKeys > un.hi || (b.window > 0 && c0 < un.lo && c0 + kPtKeys > b.sinks)) {
+          // V rows that no row of the unit sees may hold anything: their P is 0, but 0 * NaN is NaN. A warp
+          // clears its 32 keys, four rows of a 64-dim half at a time.
           ok = mbar_wait(&kv_full[2 * (J & 1) + 1], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
           if (!__all_sync(0xffffffffu, ok)) return false;
-          const int c = c0 + qrow;
-          if (c >= un.hi || (b.window > 0 && c < un.ts.lo && c >= b.sinks)) {
-            uint8_t* vr = ring + (2 * (J & 1) + 1) * kPtTile + qrow * 128;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              *reinterpret_cast<uint4*>(vr + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(vr + kPtTile / 2 + 16 * i) = make_uint4(0u, 0u, 0u, 0u);
+          uint8_t* vt = ring + (2 * (J & 1) + 1) * kPtTile + (lane & 7) * 16;
+#pragma unroll 1
+          for (int i = 0; i < 8; ++i) {
+            const int r = (warp & 3) * 32 + i * 4 + (lane >> 3), c = c0 + r;
+            if (c >= un.hi || (b.window > 0 && c < un.lo && c >= b.sinks)) {
+              *reinterpret_cast<uint4*>(vt + r * 128) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(vt + r * 128 + kPtTile / 2) = make_uint4(0u, 0u, 0u, 0u);
             }
           }
           fence_proxy_async_smem();
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&p_full[t]);
+        // P in two halves, so that the first one's MMAs run while the second is made. It goes over S's own
+        // registers, two bf16 in one, and over the first half of S's columns.
+        const float mu = m_ref == -INFINITY ? 0.f : m_ref;
+        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+          for (int c = 64 * h; c < 64 * h + 64; c += 4) {
+            float p[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              p[e] = ex2_approx(fmaf(__uint_as_float(sr[c + e]), scale, -mu));
+              rs[e] += p[e];
+            }
+            sr[c >> 1] = pack_bf16(p[0], p[1]);
+            sr[(c >> 1) + 1] = pack_bf16(p[2], p[3]);
+          }
+          tc_st32_async(s_col + 32 * h, sr + 32 * h);
+          tc_st_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(h == 0 ? &p_half[t] : &p_full[t]);
+        }
+        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
       }
       // ---- the piece's rows
       bool ok = mbar_wait(&o_done[t], (suse - 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
-      const bool whole = k0 == 0 && k1 == n;
-      const int slot = 2 * me + (at == t_begin ? 0 : 1);
-      const size_t row = (size_t)(un.token0 + token) * a.Hq + g * a.G + hj;
+      const bool whole = un.whole != 0;
+      const int slot = 2 * me + (un.first ? 0 : 1);
+      const size_t row = (size_t)(un.token0 + token) * a.Hq + un.head * a.G + hj;
       const bool has_base = a.sink.base32 != nullptr;
       RowScale rs = {1.f, 0.f, 0.f};
       if (whole && valid) rs = row_scale(m_ref, l, has_base, has_base ? a.sink.base_lse[row] : 0.f);
@@ -505,8 +595,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           float* dst = whole ? a.sink.out32 + row * kAttnD + 32 * c
                              : a.part_o + ((size_t)slot * kPtRows + t * 128 + qrow) * kAttnD + 32 * c;
 #pragma unroll
-          for (int e = 0; e < 32; e += 4)
-            *reinterpret_cast<float4*>(dst + e) = make_float4(ov[e], ov[e + 1], ov[e + 2], ov[e + 3]);
+          for (int e = 0; e < 32; e += 8) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = __float_as_uint(ov[e + i]);
+            st_global_32(dst + e, w);
+          }
         } else {
           if (has_base) {
             const float* bv = a.sink.base32 + row * kAttnD + 32 * c;
@@ -521,9 +615,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           }
           bf16* dst = a.sink.out + row * kAttnD + 32 * c;
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-            *reinterpret_cast<uint4*>(dst + e) = make_uint4(pack_bf16(ov[e], ov[e + 1]), pack_bf16(ov[e + 2], ov[e + 3]),
-                                                            pack_bf16(ov[e + 4], ov[e + 5]), pack_bf16(ov[e + 6], ov[e + 7]));
+          for (int e = 0; e < 32; e += 16) {
+            uint32_t w[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) w[i] = pack_bf16(ov[e + 2 * i], ov[e + 2 * i + 1]);
+            st_global_32(dst + e, w);
+          }
         }
       }
       if (valid) {
@@ -535,13 +632,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           a.sink.lse32[row] = rs.lse;
         }
       }
-      if (!whole && k0 == 0 && t == 0 && qrow == 0) {
+      if (un.last >= 0 && t == 0 && qrow == 0) {
         PtUnit* c = &a.cut[me];
         c->token0 = un.token0;
         c->tokens = un.tokens;
-        c->head = g;
-        c->last = tile_owner(u0 + n - 1, total, E);
-        c->first_slot = at == t_begin ? 0 : 1;
+        c->head = un.head;
+        c->last = un.last;
+        c->first_slot = un.first ? 0 : 1;
         c->valid = 1;
       }
       tc_fence_before();  // O_t is read before the next unit's MMAs write it (through p_full)

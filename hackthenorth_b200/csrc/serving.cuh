@@ -120,8 +120,8 @@ int run_paged_attention(const void* q, const void* k_pages, const void* v_pages,
                         int table_width, const int* q_start, const int* kv_lens, int n_seqs, int tokens,
                         int max_queries, int n_heads, int n_kv_heads, int window, int sinks, void* out,
                         void* workspace, size_t workspace_bytes, int* device_status, void* stream) {
-  if (!ptr_ok(k_pages) || !ptr_ok(v_pages) || !ptr_ok(workspace))
-    return set_err(nullptr, QB_ERR_ARG, "pools and workspace must be 16-byte aligned device pointers");
+  if (!ptr_ok(k_pages) || !ptr_ok(v_pages) || !ptr_ok(workspace) || (reinterpret_cast<uintptr_t>(workspace) & 255) != 0)
+    return set_err(nullptr, QB_ERR_ARG, "pools must be 16-byte and the workspace 256-byte aligned device pointers");
   if (!page_table || !q_start || !kv_lens || !device_status)
     return set_err(nullptr, QB_ERR_ARG, "page_table, q_start, kv_lens and device_status must be device pointers");
   int rc = check_heads(n_heads, n_kv_heads);
@@ -134,7 +134,8 @@ int run_paged_attention(const void* q, const void* k_pages, const void* v_pages,
   if (prefix_len > 0 && !prefix_table) return set_err(nullptr, QB_ERR_ARG, "prefix_table must be a device pointer");
   if (max_queries < 1 && tokens > 0) return set_err(nullptr, QB_ERR_ARG, "max_queries must be at least 1");
   if (tokens == 0) return QB_OK;
-  if (!ptr_ok(q) || !ptr_ok(out)) return set_err(nullptr, QB_ERR_ARG, "q and out must be 16-byte aligned device pointers");
+  if (!ptr_ok(q) || !ptr_ok(out) || (reinterpret_cast<uintptr_t>(out) & 31) != 0)
+    return set_err(nullptr, QB_ERR_ARG, "q must be a 16-byte and out a 32-byte aligned device pointer");
   if (max_queries > tokens) max_queries = tokens;
   rc = check_tiles(tokens, n_seqs, G, table_width, page_size);
   if (rc == QB_OK && prefix_len > 0) {

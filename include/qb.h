@@ -361,8 +361,8 @@ int qb_rope_paged_append(const void* qkv, const void* q_norm, const void* k_norm
 /* Workspace of qb_paged_attention (prefix_tokens 0) and
  * qb_shared_prefix_attention (prefix_tokens: its `tokens`) for calls of up to
  * max_queries; its first qb_paged_zero_bytes() bytes must be zero before its
- * first use (the kernels leave them zero). Calls that may overlap on the GPU
- * need a workspace each. */
+ * first use (the kernels leave them zero), its address a multiple of 256. Calls
+ * that may overlap on the GPU need a workspace each. */
 size_t qb_paged_zero_bytes(void);
 int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, int prefix_tokens, size_t* bytes);
 
@@ -373,7 +373,7 @@ int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, int p
  * keys that stay visible beside a window. Keys that no row sees are not read,
  * their pages included. max_queries: an upper bound of every sequence's query
  * rows (a longer sequence is reported and skipped). q, out [tokens][Hq][128]
- * bf16, q normalised and rotated. */
+ * bf16, q normalised and rotated, out 32-byte aligned. */
 int qb_paged_attention(const void* q, const void* k_pages, const void* v_pages, int num_pages, int page_size,
                        const int* page_table, int table_width, const int* q_start, const int* kv_lens, int n_seqs,
                        int tokens, int max_queries, int n_heads, int n_kv_heads, int window, int sinks, void* out,

@@ -40,7 +40,8 @@ def test_append_refuses(built_lib, kw, code):
 
 
 @pytest.mark.parametrize("kw,code", COMMON + [(dict(q=None), ARG), (dict(window=-1), ARG), (dict(sinks=-1), ARG),
-                                              (dict(max_q=-1), ARG), (dict(max_q=0), ARG), (dict(ws=None), ARG), (dict(ws_bytes=100), ARG)])
+                                              (dict(max_q=-1), ARG), (dict(max_q=0), ARG), (dict(ws=None), ARG), (dict(ws_bytes=100), ARG), (dict(out=PTR + 16), ARG),
+                                              (dict(ws=PTR + 128), ARG)])
 def test_attention_refuses(built_lib, kw, code):
     assert _attention(built_lib, **kw) == code
     assert built_lib.qb_last_error(None)
