@@ -14,7 +14,7 @@
 // each for S and P.V of a tile and M tile) and by the cache's bytes below that.
 //  * warp 0: TMA. Q tiles (3D map, 128-byte swizzle) and K and V tiles of
 //    32 KB, a box per page, into two slots each.
-//  * warp 1, one lane: the MMAs. S_t = Q_t . K^T into TMEM columns 128 t, and
+//  * warps 1 and 3: the MMAs of M tile 0 and 1. S_t = Q_t . K^T into TMEM columns 128 t, and
 //    once tile t's softmax has put P_t (bf16) over the first half of S_t,
 //    O_t += P_t . V with P_t read from TMEM into columns 256 + 128 t. S_t of the
 //    next key tile follows P_t . V in issue order, which is the order of
@@ -37,10 +37,12 @@
 
 namespace qb {
 
-constexpr int kPtKeys = 128;
+constexpr int kPtKeys = 64;
 constexpr int kPtRows = 256;
 constexpr int kPtThreads = 12 * 32;
-constexpr int kPtTile = 128 * 128 * 2;  // a Q, K or V tile: 32 KB, dims 0-63 then 64-127
+constexpr int kPtTile = 128 * 128 * 2;         // a Q tile: 32 KB, dims 0-63 then 64-127
+constexpr int kPtKvTile = kPtKeys * 128 * 2;   // a K or V tile: 16 KB, likewise
+constexpr int kPtSlots = 4;                    // ring slots of each
 constexpr int kPtMaxUnits = 7168;
 constexpr int kPtMinTiles = 2;
 
@@ -72,16 +74,40 @@ struct PagedTcArgs {
 };
 
 __host__ inline size_t pt_smem_bytes(int max_units) {
-  return 1024 + 6 * (size_t)kPtTile + 512 + kPtPieces * sizeof(PtPiece) + (size_t)(kPagedMaxSeqs + 1 + max_units + 1) * 4;
+  return 1024 + 2 * (size_t)kPtTile + 2 * kPtSlots * (size_t)kPtKvTile + 512 + kPtPieces * sizeof(PtPiece) + (size_t)(kPagedMaxSeqs + 1 + max_units + 1) * 4;
 }
 
-// d += A (TMEM) . B (shared memory)
-__device__ __forceinline__ void tc_mma_ta(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+// The MMAs as the whole warp runs them: `lead` (one lane) issues. Kept free of
+// divergence, descriptors and addresses stay in uniform registers, which the
+// instruction takes its operands from; issued from a lane's branch, every
+// operand was moved there anew, and the 32 MMAs of a key tile took longer to
+// issue (5000 cycles) than to run (2048).
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t r;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+  return r != 0;
+}
+__device__ __forceinline__ void tc_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %6, %7, %8}, p;\n\t}"
-      ::"r"(tmem_d), "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(acc), "r"(0u), "r"(0u), "r"(0u), "r"(0u)
+      "{\n\t.reg .pred p, l;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 l, %5, 0;\n\t"
+      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void tc_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+  asm volatile(
+      "{\n\t.reg .pred p, l;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 l, %5, 0;\n\t"
+      "@l tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void tc_commit_by(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred l;\n\tsetp.ne.b32 l, %1, 0;\n\t"
+      "@l tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
       : "memory");
 }
 // 32 columns of this warp's lanes without the wait (tc_ld_wait follows).
@@ -119,6 +145,45 @@ __device__ __forceinline__ void st_global_32(void* p, const uint32_t (&w)[8]) {
   asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
                "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
                : "memory");
+}
+
+// mbar_wait with a short path for the polls that the kernel's rarer roles make:
+// their code is fetched anew each time, so its length counts.
+__device__ __forceinline__ bool pt_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  if (mbar_try_wait(bar, parity)) return true;
+  const unsigned long long t0 = global_timer_ns();
+#pragma unroll 1
+  while (!mbar_try_wait(bar, parity))
+    if (global_timer_ns() - t0 > kWaitLimitNs) {
+      report_error(err, code);
+      return false;
+    }
+  return true;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
+}
+// Two fp32 values in one register pair, for sm_100's packed arithmetic.
+__device__ __forceinline__ uint64_t f32x2(float a, float b) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ void unpack_f32x2(uint64_t v, float& a, float& b) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma_f32x2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
 // A word with its lowest n bits set (n clamped to 0..32).
@@ -179,46 +244,48 @@ __global__ void __launch_bounds__(kPtThreads, 1)
                     const __grid_constant__ CUtensorMap tmv, const PagedTcArgs a) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* qs = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = qs + 2 * kPtTile;  // K, V, K, V
-  uint64_t* bars = reinterpret_cast<uint64_t*>(ring + 4 * kPtTile);
-  uint64_t* kv_full = bars;        // [4]
-  uint64_t* kv_empty = bars + 4;   // [4]
-  uint64_t* q_full = bars + 8;     // [2]
-  uint64_t* q_empty = bars + 10;   // [2]
-  uint64_t* s_full = bars + 12;    // [2]
-  uint64_t* p_half = bars + 14;    // [2] P of the tile's keys 0-63
-  uint64_t* p_full = bars + 16;    // [2] P of all of them
-  uint64_t* o_done = bars + 18;    // [2]
-  uint64_t* piece_full = bars + 20;   // [4]
-  uint64_t* piece_empty = bars + 24;  // [4]
-  uint64_t* done = bars + 28;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 29);
+  uint8_t* kring = qs + 2 * kPtTile;
+  uint8_t* vring = kring + kPtSlots * kPtKvTile;
+  uint64_t* bars = reinterpret_cast<uint64_t*>(vring + kPtSlots * kPtKvTile);
+  uint64_t* kv_full = bars;            // [2][slots]: K, V
+  uint64_t* kv_empty = bars + 8;       // [2][slots]
+  uint64_t* q_full = bars + 16;        // [2]
+  uint64_t* q_empty = bars + 18;       // [2]
+  uint64_t* s_full = bars + 20;        // [2 M tiles][2 buffers]
+  // of S's buffers too: P may be a tile ahead of its MMAs, which are then two phases of one barrier behind
+  uint64_t* p_full = bars + 24;        // [2][2]
+  uint64_t* o_done = bars + 28;        // [2][2]
+  uint64_t* done = bars + 32;          // [2]
+  uint64_t* piece_full = bars + 34;    // [4]
+  uint64_t* piece_empty = bars + 38;   // [4]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 42);
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* warp_tot = reinterpret_cast<int*>(tmem_slot + 2);  // [12]
   PtPiece* pieces = reinterpret_cast<PtPiece*>(bars + 64);
   int* seq_unit = reinterpret_cast<int*>(pieces + kPtPieces);  // [n_seqs + 1] units before each sequence
   int* unit_tile = seq_unit + kPagedMaxSeqs + 1;          // [units + 1] tiles before each unit
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
   const int RH = 128 / a.G;  // tokens per M tile
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < 4; ++s) {
+    for (int s = 0; s < 2 * kPtSlots; ++s) {
       mbar_init(&kv_full[s], 1);
-      mbar_init(&kv_empty[s], 1);
+      mbar_init(&kv_empty[s], 2);
     }
     for (int t = 0; t < 2; ++t) {
       mbar_init(&q_full[t], 1);
       mbar_init(&q_empty[t], 1);
-      mbar_init(&s_full[t], 1);
-      mbar_init(&p_half[t], 4);
-      mbar_init(&p_full[t], 4);
-      mbar_init(&o_done[t], 1);
+      for (int i = 2 * t; i < 2 * t + 2; ++i) {
+        mbar_init(&s_full[i], 1);
+        mbar_init(&p_full[i], 4);
+        mbar_init(&o_done[i], 1);
+      }
+      mbar_init(&done[t], 1);
     }
-    mbar_init(done, 1);
     for (int i = 0; i < kPtPieces; ++i) {
       mbar_init(&piece_full[i], 1);
-      mbar_init(&piece_empty[i], 10);  // producer, MMA issuer, 8 softmax warps
+      mbar_init(&piece_empty[i], 11);  // producer, 2 MMA warps, 8 softmax warps
     }
     fence_mbar_init();
     flags[0] = 0;
@@ -270,17 +337,20 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   __syncthreads();
 
   // Every role takes the same pieces in turn: f(piece), until an empty one. Lane 0 frees the entry.
-  auto walk = [&](uint32_t lanes_of_role, auto&& f) {
+  auto walk = [&](auto&& f, auto&& gave_up) {
     for (int i = 0;; ++i) {
       const int e = i % kPtPieces;
-      if (!mbar_wait(&piece_full[e], (i / kPtPieces) & 1, a.err, DEV_TIMEOUT_ATTN_FULL)) return;
+      if (!__all_sync(0xffffffffu, mbar_wait(&piece_full[e], (i / kPtPieces) & 1, a.err, DEV_TIMEOUT_ATTN_FULL))) {
+        gave_up();
+        return;
+      }
       union {
         uint4 w[4];
         PtPiece p;
       } u;
 #pragma unroll
       for (int j = 0; j < 4; ++j) u.w[j] = reinterpret_cast<const uint4*>(&pieces[e])[j];
-      __syncwarp(lanes_of_role);
+      __syncwarp();
       if (lane == 0) mbar_arrive(&piece_empty[e]);
       if (u.p.k0 == u.p.k1 || !f(u.p)) return;
     }
@@ -288,14 +358,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   auto tile_key = [&](const PtPiece& p, int k) { return (k < p.n_sink ? k : k - p.n_sink + p.lo_tile) * kPtKeys; };
 
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0) {
       // -------------------------------------------------------------- producer
       const int br = min(1 << b.page_log2, kPtKeys), nbox = kPtKeys / br;
       const int kind = lane & 3, box = lane >> 2;
       int issued = 0, quse[2] = {0, 0};
       bool ok = true;
-      walk(0xffffffffu, [&](const PtPiece& un) {
+      walk([&](const PtPiece& un) {
         const int g = un.head, k0 = un.k0, k1 = un.k1;
         auto page_of = [&](int k) {
           const int c0 = tile_key(un, k) + box * br;
@@ -324,30 +393,31 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           page = page_of(k + 1);  // its load runs while the slots are waited for
           const int y = ((now * a.Hkv + g) << b.page_log2) + (c0 & ((1 << b.page_log2) - 1));
           const uint32_t bytes = __popc(__ballot_sync(0xffffffffu, now >= 0 && kind < 2)) * br * 128;
+          const int slot = issued % kPtSlots, parity = ((issued / kPtSlots) - 1) & 1;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            const int s = 2 * (issued & 1) + kv;
-            if (issued >= 2)
-              ok = ok && __all_sync(0xffffffffu, mbar_wait(&kv_empty[s], ((issued >> 1) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY));
+            uint64_t* full = &kv_full[kv * kPtSlots + slot];
+            if (issued >= kPtSlots)
+              ok = ok && __all_sync(0xffffffffu, mbar_wait(&kv_empty[kv * kPtSlots + slot], parity, a.err, DEV_TIMEOUT_ATTN_EMPTY));
             if (!ok) break;
-            if (lane == 0) mbar_arrive_expect_tx(&kv_full[s], bytes);
+            if (lane == 0) mbar_arrive_expect_tx(full, bytes);
             __syncwarp();
             if (now >= 0 && (kind >> 1) == kv)
-              tma_load_2d(ring + s * kPtTile + (kind & 1) * (kPtTile / 2) + box * br * 128, kv ? &tmv : &tmk,
-                          64 * (kind & 1), y, &kv_full[s]);
+              tma_load_2d((kv ? vring : kring) + slot * kPtKvTile + (kind & 1) * (kPtKvTile / 2) + box * br * 128,
+                          kv ? &tmv : &tmk, 64 * (kind & 1), y, full);
           }
           if (ok) ++issued;
         }
         if (flags[0] != 0) ok = false;
         return ok;
-      });
+      }, [&] { ok = false; });
       if (!ok) flags[0] = 1;
       // keep shared memory alive until every issued copy has landed (after a failure a K tile may have no V: the
       // waits are bounded)
       for (int t = 0; t < 2; ++t)
         if (quse[t] > 0) mbar_wait(&q_full[t], (quse[t] - 1) & 1, nullptr, 0);
-      for (int i = max(0, issued - 2); i < issued + (ok ? 0 : 1); ++i)
-        for (int kv = 0; kv < 2; ++kv) mbar_wait(&kv_full[2 * (i & 1) + kv], (i >> 1) & 1, nullptr, 0);
+      for (int i = max(0, issued - kPtSlots); i < issued + (ok ? 0 : 1); ++i)
+        for (int kv = 0; kv < 2; ++kv) mbar_wait(&kv_full[kv * kPtSlots + i % kPtSlots], (i / kPtSlots) & 1, nullptr, 0);
     } else if (warp == 2 && lane == 0) {
       // ------------------------------------------------------------- scheduler
       int u = 0;
@@ -395,73 +465,85 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         mbar_arrive(&piece_full[e]);
         if (p.k0 == p.k1 || flags[0] != 0) break;
       }
-    } else if (warp == 1 && lane == 0) {
+    } else if (warp == 1 || warp == 3) {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t idesc_s = pg_idesc(128, kPtKeys);
       const uint32_t idesc_o = pg_idesc(128, 128) | (1u << 16);  // B (V) MN-major
       // descriptors made once; an offset of x bytes adds x >> 4 (the addresses stay below 2^18)
-      const uint64_t qd = ft_desc(qs, 16, 1024), kd = ft_desc(ring, 16, 1024);
-      const uint64_t vd = ft_desc(ring + kPtTile, kPtTile / 2, 1024);
-      int J = 0, quse[2] = {0, 0}, puse[2] = {0, 0};
+      const uint64_t qd = ft_desc(qs, 16, 1024), kd = ft_desc(kring, 16, 1024);
+      const uint64_t vd = ft_desc(vring, kPtKvTile / 2, 1024);
+      const uint32_t lead = elect_lane() ? 1u : 0u;
+      const int t = warp == 1 ? 0 : 1;
+      auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+      auto wait = [&](uint64_t* bar, int parity) {
+        return __all_sync(0xffffffffu, pt_wait(bar, parity, a.err, DEV_TIMEOUT_ATTN_FULL)) != 0;
+      };
+      const uint64_t qt = qd + (uint64_t)(t * (kPtTile >> 4));
+      const uint32_t sd = tmem + (uint32_t)(128 * t), od = tmem + (uint32_t)(256 + 128 * t);
+      int J = 0, qphase = 0, pphase = 0;
       bool ok = true;
-      walk(1u, [&](const PtPiece& un) {
-        const int k0 = un.k0, k1 = un.k1;
-        const int nt = un.tokens > RH ? 2 : 1;
-        auto issue_s = [&](int t, int j) {  // S_t of key tile j of this CTA
-          const uint64_t qt = qd + (uint64_t)(t * (kPtTile >> 4)), kt = kd + (uint64_t)((j & 1) * (2 * kPtTile >> 4));
-#pragma unroll
-          for (int k = 0; k < 8; ++k)  // 16 dims a step
-            tc_mma(tmem + (uint32_t)(t * 128), qt + (k >> 2) * (kPtTile >> 5) + (k & 3) * 2,
-                   kt + (k >> 2) * (kPtTile >> 5) + (k & 3) * 2, idesc_s, k > 0 ? 1u : 0u);
-          tc_commit(&s_full[t]);
-        };
-        ok = ok && mbar_wait(&kv_full[2 * (J & 1)], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
-        for (int t = 0; t < nt && ok; ++t) {
-          ok = mbar_wait(&q_full[t], quse[t] & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
-          if (!ok) break;
-          ++quse[t];
-          tc_fence_after();
-          issue_s(t, J);
-          if (k1 - k0 == 1) tc_commit(&q_empty[t]);
+      walk([&](const PtPiece& un) {
+        const int n = uniform(un.k1 - un.k0);
+        const bool both = uniform(un.tokens > RH) != 0;
+        if (t == 1 && !both) {
+          J += n;
+          return true;
         }
-        if (ok) tc_commit(&kv_empty[2 * (J & 1)]);
-        for (int k = k0; k < k1 && ok; ++k, ++J) {
-          const uint64_t vt = vd + (uint64_t)((J & 1) * (2 * kPtTile >> 4));
-          ok = mbar_wait(&kv_full[2 * (J & 1) + 1], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
-          for (int t = 0; t < nt && ok; ++t) {
-            const uint32_t od = tmem + (uint32_t)(256 + 128 * t), pd = tmem + (uint32_t)(128 * t);
-            ok = mbar_wait(&p_half[t], puse[t] & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
-            if (!ok) break;
-            tc_fence_after();
+        auto full = [&](int kv, int j) { return wait(&kv_full[kv * kPtSlots + j % kPtSlots], (j / kPtSlots) & 1); };
+        // a slot is free after both M tiles' MMAs; of a lone tile it is released twice
+        auto release = [&](int kv, int j) {
+          tc_commit_by(lead, &kv_empty[kv * kPtSlots + j % kPtSlots]);
+          if (!both) tc_commit_by(lead, &kv_empty[kv * kPtSlots + j % kPtSlots]);
+        };
+        auto issue_s = [&](int j) {  // S_t of key tile j of this CTA into buffer j & 1: 16 dims a step
+          const uint64_t kt = kd + (uint64_t)((j % kPtSlots) * (kPtKvTile >> 4));
 #pragma unroll
-            for (int ks = 0; ks < 4; ++ks)  // 16 keys a step
-              tc_mma_ta(od, pd + 8 * ks, vt + ks * 128, idesc_o, (k > k0 || ks > 0) ? 1u : 0u);
-            ok = mbar_wait(&p_full[t], puse[t] & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
-            if (!ok) break;
-            ++puse[t];
-            tc_fence_after();
+          for (int k = 0; k < 8; ++k)
+            tc_mma_ss(lead, sd + (uint32_t)(64 * (j & 1)), qt + (k >> 2) * (kPtTile >> 5) + (k & 3) * 2,
+                      kt + (k >> 2) * (kPtKvTile >> 5) + (k & 3) * 2, idesc_s, k > 0 ? 1u : 0u);
+          tc_commit_by(lead, &s_full[2 * t + (j & 1)]);
+          release(0, j);
+        };
+        ok = wait(&q_full[t], qphase) && full(0, J);
+        if (!ok) return false;
+        qphase ^= 1;
+        tc_fence_after();
+        issue_s(J);
+        if (n > 1) {
+          ok = full(0, J + 1);
+          if (!ok) return false;
+          tc_fence_after();
+          issue_s(J + 1);
+        }
+        if (n <= 2) tc_commit_by(lead, &q_empty[t]);
+        ok = full(1, J) && (n <= 2 || full(0, J + 2));
+#pragma unroll 1
+        for (int k = 0; k < n && ok; ++k, ++J) {
+          ok = wait(&p_full[2 * t + (J & 1)], (pphase >> (J & 1)) & 1);
+          if (!ok) break;
+          pphase ^= 1 << (J & 1);
+          tc_fence_after();
+          // O_t += P_t . V: 16 keys a step, P in the first half of S's buffer
+          const uint64_t vt = vd + (uint64_t)((J % kPtSlots) * (kPtKvTile >> 4));
 #pragma unroll
-            for (int ks = 4; ks < 8; ++ks) tc_mma_ta(od, pd + 8 * ks, vt + ks * 128, idesc_o, 1u);
-            tc_commit(&o_done[t]);
-            if (t == nt - 1) tc_commit(&kv_empty[2 * (J & 1) + 1]);
-            if (k + 1 < k1) {
-              if (t == 0) ok = mbar_wait(&kv_full[2 * ((J + 1) & 1)], ((J + 1) >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
-              if (!ok) break;
-              tc_fence_after();
-              issue_s(t, J + 1);
-              if (k + 2 == k1) tc_commit(&q_empty[t]);
-              if (t == nt - 1) tc_commit(&kv_empty[2 * ((J + 1) & 1)]);
-            }
+          for (int i = 0; i < 4; ++i)
+            tc_mma_ts(lead, od, sd + (uint32_t)(64 * (J & 1) + 8 * i), vt + i * 128, idesc_o, i > 0 || k > 0 ? 1u : 0u);
+          tc_commit_by(lead, &o_done[2 * t + (J & 1)]);
+          release(1, J);
+          if (k + 2 < n) {
+            issue_s(J + 2);  // over P's buffer: runs after P . V, as issued
+            if (k + 3 == n) tc_commit_by(lead, &q_empty[t]);
           }
+          // what the next pass needs, waited for under this one's MMAs
+          if (k + 1 < n) ok = full(1, J + 1) && (k + 3 >= n || full(0, J + 3));
         }
         return ok;
-      });
+      }, [&] { ok = false; });
       if (!ok) flags[0] = 1;
-      tc_commit(done);  // TMEM is released below only after every MMA issued here has completed
-      mbar_wait(done, 0, nullptr, 0);
+      tc_commit_by(lead, &done[t]);  // TMEM is released below only after every MMA issued here has completed
+      mbar_wait(&done[t], 0, nullptr, 0);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
     // ----------------------------------------------------------------- softmax
     const int t = (warp - 4) >> 2;  // M tile
     const int qrow = (warp & 3) * 32 + lane;
@@ -469,8 +551,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
     const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16;
     const uint32_t s_col = tmem + lanes + 128 * t, o_col = tmem + lanes + 256 + 128 * t;
     const float scale = kLog2e * 0.08838834764831845f;  // log2(e) / sqrt(128)
-    int J = 0, suse = 0;
-    walk(0xffffffffu, [&](const PtPiece& un) {
+    int J = 0;
+    uint32_t sphase = 0;  // of S's two buffers: the phase of their next use
+    // O_t with key tile j, the last one whose S was read in its buffer, added
+    auto pv_done = [&](int j) {
+      return mbar_wait(&o_done[2 * t + (j & 1)], ((sphase >> (j & 1)) & 1) ^ 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+    };
+    walk([&](const PtPiece& un) {
       const int k0 = un.k0, k1 = un.k1;
       if (t * RH >= un.tokens) {
         J += k1 - k0;
@@ -480,14 +567,16 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const bool valid = qi < RH && token < un.tokens;
       const int pos = !valid ? -1 : b.q_start == nullptr ? un.hi - 1 : un.p_first + token;
       float m_ref = -INFINITY, l = 0.f;
-      for (int k = k0; k < k1; ++k, ++J, ++suse) {
+      for (int k = k0; k < k1; ++k, ++J) {
         const int c0 = tile_key(un, k);
-        bool ok = mbar_wait(&s_full[t], suse & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
+        const uint32_t buf = s_col + 64 * (J & 1);
+        bool ok = mbar_wait(&s_full[2 * t + (J & 1)], (sphase >> (J & 1)) & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
         if (!__all_sync(0xffffffffu, ok)) return false;
+        sphase ^= 1u << (J & 1);
         tc_fence_after();
-        uint32_t sr[128];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tc_ld32_async(s_col + 32 * c, sr + 32 * c);
+        uint32_t sr[64];
+        tc_ld32_async(buf, sr);
+        tc_ld32_async(buf + 32, sr + 32);
         tc_ld_wait(sr);
         // keys [lo, hi) and [0, first) of the tile are visible to this row
         const int hi = pos - c0 + 1;
@@ -495,24 +584,25 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int first = b.sinks - c0;
         if (!__all_sync(0xffffffffu, hi >= kPtKeys && (lo <= 0 || first >= kPtKeys))) {
 #pragma unroll
-          for (int w = 0; w < 4; ++w) {  // one bit a key, so that each score costs a test and a select
+          for (int w = 0; w < 2; ++w) {  // one bit a key, so that each score costs a test and a select
             const uint32_t seen = bits_below(hi - 32 * w) & (~bits_below(lo - 32 * w) | bits_below(first - 32 * w));
 #pragma unroll
             for (int c = 0; c < 32; ++c)  // -inf where unseen, whatever the score was
               sr[32 * w + c] = (seen >> c) & 1u ? sr[32 * w + c] : 0xff800000u;
           }
         }
-        float mx[8];
+        float mx[4];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) mx[e] = __uint_as_float(sr[e]);
+        for (int e = 0; e < 4; ++e) mx[e] = fmaxf(__uint_as_float(sr[e]), __uint_as_float(sr[e + 4]));
 #pragma unroll
-        for (int c = 8; c < 128; ++c) mx[c & 7] = fmaxf(mx[c & 7], __uint_as_float(sr[c]));
-        const float m_new = scale * fmaxf(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])),
-                                          fmaxf(fmaxf(mx[4], mx[5]), fmaxf(mx[6], mx[7])));
+        for (int c = 8; c < 64; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) mx[e] = max3(mx[e], __uint_as_float(sr[c + e]), __uint_as_float(sr[c + e + 4]));
+        const float m_new = scale * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
         // A row that has seen nothing has O = l = 0: its reference moves freely.
         if (m_ref == -INFINITY) m_ref = m_new;
         if (__any_sync(0xffffffffu, m_new > m_ref + 8.f)) {
-          ok = mbar_wait(&o_done[t], (suse - 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          ok = pv_done(J - 1);
           if (!__all_sync(0xffffffffu, ok)) return false;
           tc_fence_after();
           const float top = fmaxf(m_ref, m_new);
@@ -535,47 +625,45 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         }
         if (c0 + kPtKeys > un.hi || (b.window > 0 && c0 < un.lo && c0 + kPtKeys > b.sinks)) {
           // V rows that no row of the unit sees may hold anything: their P is 0, but 0 * NaN is NaN. A warp
-          // clears its 32 keys, four rows of a 64-dim half at a time.
-          ok = mbar_wait(&kv_full[2 * (J & 1) + 1], (J >> 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          // clears 16 keys, four rows of a 64-dim half at a time.
+          ok = mbar_wait(&kv_full[kPtSlots + J % kPtSlots], (J / kPtSlots) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
           if (!__all_sync(0xffffffffu, ok)) return false;
-          uint8_t* vt = ring + (2 * (J & 1) + 1) * kPtTile + (lane & 7) * 16;
+          uint8_t* vt = vring + (J % kPtSlots) * kPtKvTile + (lane & 7) * 16;
 #pragma unroll 1
-          for (int i = 0; i < 8; ++i) {
-            const int r = (warp & 3) * 32 + i * 4 + (lane >> 3), c = c0 + r;
+          for (int i = 0; i < 4; ++i) {
+            const int r = (warp & 3) * 16 + i * 4 + (lane >> 3), c = c0 + r;
             if (c >= un.hi || (b.window > 0 && c < un.lo && c >= b.sinks)) {
               *reinterpret_cast<uint4*>(vt + r * 128) = make_uint4(0u, 0u, 0u, 0u);
-              *reinterpret_cast<uint4*>(vt + r * 128 + kPtTile / 2) = make_uint4(0u, 0u, 0u, 0u);
+              *reinterpret_cast<uint4*>(vt + r * 128 + kPtKvTile / 2) = make_uint4(0u, 0u, 0u, 0u);
             }
           }
           fence_proxy_async_smem();
         }
-        // P in two halves, so that the first one's MMAs run while the second is made. It goes over S's own
-        // registers, two bf16 in one, and over the first half of S's columns.
+        // P over S's own registers, two bf16 in one, and over the first half of the buffer.
         const float mu = m_ref == -INFINITY ? 0.f : m_ref;
-        float rs[4] = {0.f, 0.f, 0.f, 0.f};
+        const uint64_t scale2 = f32x2(scale, scale), mu2 = f32x2(-mu, -mu);
+        uint64_t rs[2] = {0ull, 0ull};
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-#pragma unroll
-          for (int c = 64 * h; c < 64 * h + 64; c += 4) {
-            float p[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              p[e] = ex2_approx(fmaf(__uint_as_float(sr[c + e]), scale, -mu));
-              rs[e] += p[e];
-            }
-            sr[c >> 1] = pack_bf16(p[0], p[1]);
-            sr[(c >> 1) + 1] = pack_bf16(p[2], p[3]);
-          }
-          tc_st32_async(s_col + 32 * h, sr + 32 * h);
-          tc_st_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(h == 0 ? &p_half[t] : &p_full[t]);
+        for (int c = 0; c < 64; c += 2) {
+          const uint64_t x = fma_f32x2(f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, mu2);
+          float p0, p1;
+          unpack_f32x2(x, p0, p1);
+          p0 = ex2_approx(p0);
+          p1 = ex2_approx(p1);
+          rs[(c >> 1) & 1] = add_f32x2(rs[(c >> 1) & 1], f32x2(p0, p1));
+          sr[c >> 1] = pack_bf16(p0, p1);
         }
-        l += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+        tc_st32_async(buf, sr);
+        tc_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&p_full[2 * t + (J & 1)]);
+        float r0, r1;
+        unpack_f32x2(add_f32x2(rs[0], rs[1]), r0, r1);
+        l += r0 + r1;
       }
       // ---- the piece's rows
-      bool ok = mbar_wait(&o_done[t], (suse - 1) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+      const bool ok = pv_done(J - 1);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
       const bool whole = un.whole != 0;
@@ -643,7 +731,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       }
       tc_fence_before();  // O_t is read before the next unit's MMAs write it (through p_full)
       return true;
-    });
+    }, [] {});
   }
   tc_fence_before();
   __syncthreads();
