@@ -79,6 +79,8 @@ SIGNATURES = {
                            + [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "qb_shared_prefix_attention": (c_int, [c_void_p] * 3 + [c_int] * 2 + [c_void_p, c_int, c_int, c_void_p, c_int]
                                    + [c_void_p] * 2 + [c_int] * 5 + [c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "qb_sample_token": (c_int, [c_void_p, c_int, c_int, c_int, c_void_p, c_void_p, c_float, c_void_p, c_int, c_void_p,
+                                c_float, c_void_p, c_float, c_void_p, c_void_p, c_void_p]),
     "qb_op_check": (c_int, [c_void_p, c_void_p]),
     "qb_grouped_attention_noalloc": (c_int, [c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p,
                                              c_void_p, c_void_p, c_void_p]),

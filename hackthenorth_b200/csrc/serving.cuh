@@ -4,6 +4,7 @@
 #pragma once
 #include "paged_attention_tc.cuh"
 #include "paged_decode.cuh"
+#include "sample.cuh"
 
 namespace {
 
@@ -222,6 +223,16 @@ int run_paged_attention(const void* q, const void* k_pages, const void* v_pages,
   return QB_OK;
 }
 
+template <typename T>
+cudaError_t launch_sample(SampleArgs a, int rows, cudaStream_t st) {
+  static bool set[kMaxDevices] = {};
+  a.slice = (int)align_up((a.vocab + kSmCluster - 1) / kSmCluster, kSmWarps * 8);
+  cudaError_t e = smem_attr(sample_kernel<T>, set, sample_smem_bytes(kSmMaxVocab / kSmCluster, sizeof(T)));
+  if (e != cudaSuccess) return e;
+  return launch_ex(sample_kernel<T>, dim3((unsigned)rows * kSmCluster), dim3(kSmThreads),
+                   sample_smem_bytes(a.slice, sizeof(T)), st, a);
+}
+
 }  // namespace
 
 extern "C" {
@@ -300,6 +311,35 @@ int qb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
   return run_paged_attention(q, k_pages, v_pages, num_pages, page_size, prefix_table, prefix_pages, prefix_len,
                              page_table, table_width, q_start, kv_lens, n_seqs, tokens, max_queries, n_heads, n_kv_heads,
                              0, 0, out, workspace, workspace_bytes, device_status, stream);
+}
+
+int qb_sample_token(const void* logits, int fp32, int rows, int vocab, const float* uniforms, const float* temperature,
+                    float temperature_all, const int* top_k, int top_k_all, const float* top_p, float top_p_all,
+                    const float* min_p, float min_p_all, int64_t* token_out, int* device_status, void* stream) {
+  if (rows < 0 || rows > (1 << 24)) return set_err(nullptr, QB_ERR_UNSUPPORTED, "0..2^24 rows");
+  if (vocab < 1 || vocab > kSmMaxVocab) return set_err(nullptr, QB_ERR_UNSUPPORTED, "vocab must lie in 1..262144");
+  if (rows == 0) return QB_OK;
+  if (!logits || (reinterpret_cast<uintptr_t>(logits) & (fp32 ? 3 : 1)) != 0 || !uniforms || !token_out || !device_status)
+    return set_err(nullptr, QB_ERR_ARG, "logits, uniforms, token_out and device_status must be device pointers");
+  SampleArgs a;
+  std::memset(&a, 0, sizeof(a));
+  a.logits = logits;
+  a.uniforms = uniforms;
+  a.temperature = temperature;
+  a.top_k = top_k;
+  a.top_p = top_p;
+  a.min_p = min_p;
+  a.temperature_all = temperature_all;
+  a.top_k_all = top_k_all;
+  a.top_p_all = top_p_all;
+  a.min_p_all = min_p_all;
+  a.vocab = vocab;
+  a.out = token_out;
+  a.err = device_status;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  cudaError_t e = fp32 ? launch_sample<float>(a, rows, st) : launch_sample<bf16>(a, rows, st);
+  if (e != cudaSuccess) return cuda_fail(nullptr, e, "sample launch");
+  return QB_OK;
 }
 
 }  // extern "C"

@@ -338,3 +338,48 @@ def _paged_bytes(max_queries, hq, hkv, prefix_tokens) -> int:
     n = _lib.c_size_t()
     _lib.check(_lib.load().qb_paged_workspace_bytes(max_queries, hq, hkv, prefix_tokens, _lib.ctypes.byref(n)))
     return n.value
+
+
+def _setting(value, name, rows, dtype, device, lo, hi):
+    """(device address or None, number) of a sampling setting: one number for all rows, or a tensor [rows]."""
+    if torch.is_tensor(value):
+        _require(value.dtype == dtype and value.device == device and value.is_contiguous() and value.numel() == rows,
+                 f"{name} must be a number or a contiguous {dtype} tensor [rows] on the device of the logits")
+        return value.data_ptr(), 0
+    _require(lo <= value <= hi, f"{name} must lie in [{lo}, {hi}]")
+    return None, value
+
+
+def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+    """Draw one token per row: temperature, then top-k, top-p and min-p, from given uniform numbers.
+
+    logits ``[R, V]`` (or ``[V]``) bf16 or fp32, V at most 262144; uniforms
+    fp32 ``[R]`` in [0, 1) -> int64 ``[R]``. Every setting is a number or a
+    tensor ``[R]`` (fp32; top_k int32). Tokens rank by falling logit, then
+    rising index; ``top_k`` > 0 keeps the first ranks, ``top_p`` < 1 of these
+    the ones before which less than ``top_p`` of their mass lies, ``min_p`` > 0
+    of these the ones with at least ``min_p`` of the largest weight; the token
+    is the first, by index, at which the kept mass passes ``uniform`` times the
+    whole. Temperature 0 takes the largest logit, lowest index on ties, as
+    ``greedy_token``. A row without a finite logit gives -1 and raises in
+    ``check_device_errors``. The sampled counterpart of
+    ``dryft/engine/kernels/greedy.py:45-60``."""
+    _require(logits.is_cuda and logits.dtype in (BF16, torch.float32) and logits.is_contiguous() and logits.dim() in (1, 2),
+             "expected contiguous bf16 or fp32 CUDA logits [R, V]")
+    dev, vocab = logits.device, logits.shape[-1]
+    rows = 1 if logits.dim() == 1 else logits.shape[0]
+    _require(uniforms.dtype == torch.float32 and uniforms.device == dev and uniforms.is_contiguous()
+             and uniforms.numel() == rows, "uniforms must be a contiguous fp32 tensor [R] on the device of the logits")
+    t, t_all = _setting(temperature, "temperature", rows, torch.float32, dev, 0.0, float("inf"))
+    k, k_all = _setting(top_k, "top_k", rows, torch.int32, dev, 0, 2 ** 31 - 1)
+    p, p_all = _setting(top_p, "top_p", rows, torch.float32, dev, 0.0, 1.0)
+    m, m_all = _setting(min_p, "min_p", rows, torch.float32, dev, 0.0, 1.0)
+    with _on(dev):
+        if out is None:
+            out = torch.empty(rows, dtype=torch.int64, device=dev)
+        _require(out.dtype == torch.int64 and out.device == dev and out.is_contiguous() and out.numel() == rows,
+                 "out must be a contiguous int64 tensor [R] on the device of the logits")
+        _lib.check(_lib.load().qb_sample_token(logits.data_ptr(), int(logits.dtype == torch.float32), rows, vocab,
+                                               uniforms.data_ptr(), t, t_all, k, k_all, p, p_all, m, m_all,
+                                               out.data_ptr(), _status(dev), _lib.stream_handle()))
+    return out

@@ -392,6 +392,23 @@ int qb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
                                int max_queries, int n_heads, int n_kv_heads, void* out, void* workspace,
                                size_t workspace_bytes, int* device_status, void* stream);
 
+/* Draw one token per row of logits ([rows][vocab], bf16, or fp32 when fp32 is
+ * not 0; vocab at most 262144) from the row's uniform number in [0, 1): the
+ * sampled counterpart of greedy_token (dryft/engine/kernels/greedy.py:45-60).
+ * With w_i = exp((x_i - max x) / temperature) and tokens ranked by falling
+ * logit, then rising index: top_k > 0 keeps the first top_k ranks, top_p < 1 of
+ * these the ranks before which less than top_p of their mass lies (the first
+ * always), min_p > 0 of these the tokens with w_i >= min_p. The token is the
+ * first, by index, at which the kept tokens' running mass exceeds uniform times
+ * their mass. temperature 0 (or below): the largest logit's lowest index. Each
+ * setting is a device array [rows] or, where that is NULL, the value beside it
+ * for all rows. Logits of -inf and NaN are never drawn; a row of nothing else
+ * gives -1 and is reported. Masses are summed as integers: the result does not
+ * depend on the order of execution. */
+int qb_sample_token(const void* logits, int fp32, int rows, int vocab, const float* uniforms, const float* temperature,
+                    float temperature_all, const int* top_k, int top_k_all, const float* top_p, float top_p_all,
+                    const float* min_p, float min_p_all, int64_t* token_out, int* device_status, void* stream);
+
 /* Read the device error word of an op-level scratch (synchronises stream). */
 int qb_op_check(void* scratch, void* stream);
 

@@ -85,3 +85,17 @@ def test_python_calls_refuse_cpu_tensors():
     with pytest.raises(ValueError):
         ops.rope_paged_append(torch.zeros(1, 4096, dtype=torch.bfloat16), None, None, z[0, 0], z[0, 0], z, z, i[None], i,
                               i[:1])
+
+
+@pytest.mark.parametrize("kw,code", [(dict(logits=None), ARG), (dict(logits=PTR + 1), ARG), (dict(fp32=1, logits=PTR + 2), ARG),
+                                     (dict(uniforms=None), ARG), (dict(out=None), ARG), (dict(status=None), ARG),
+                                     (dict(rows=-1), UNSUPPORTED), (dict(vocab=0), UNSUPPORTED),
+                                     (dict(vocab=262145), UNSUPPORTED)])
+def test_sample_refuses(built_lib, kw, code):
+    a = dict(logits=PTR, fp32=0, rows=1, vocab=100, uniforms=PTR, t=None, t_all=1.0, k=None, k_all=0, p=None, p_all=1.0,
+             m=None, m_all=0.0, out=PTR, status=PTR, stream=None)
+    a.update(kw)
+    assert built_lib.qb_sample_token(*a.values()) == code
+    assert built_lib.qb_last_error(None)
+    a.update(logits=None, rows=0, vocab=100)
+    assert built_lib.qb_sample_token(*a.values()) == 0
