@@ -21,7 +21,9 @@
 //     1/32 each (the last takes the rest): monotone in x, and unlike bins of
 //     x's own bits not a handful of crowded ones. Each CTA sums its share of the
 //     bins over the cluster and finds whether the border lies there.
-//  3. the border's bin again in 1024 sub-bins; a sub-bin whose tokens are not
+//  3. up to 4096 tokens in the bins up to the border's (nearly always): put in a
+//     list, and one CTA finds the border among them
+//     else: the border's bin again in 1024 sub-bins; a sub-bin whose tokens are not
 //     all equal is split by 8 bits of the value's ordered pattern at a time
 //  4. the kept mass of every warp's stretch of indexes, the stretch that the
 //     target falls in, the token in it
@@ -60,16 +62,36 @@ struct SampleBorder {  // the slot that holds the last kept rank
   unsigned found;
 };
 
+constexpr int kSmList = 4096;  // tokens of a list
+constexpr int kSmShort = 256;  // of one whose ranks are counted token by token
+
 struct alignas(16) SampleShared {
-  unsigned cnt[kSmBins], lo[kSmBins], hi[kSmBins], kor[kSmBins], kand[kSmBins];
+  union {
+    struct {
+      unsigned cnt[kSmBins], lo[kSmBins], hi[kSmBins], kor[kSmBins], kand[kSmBins];
+    };
+    struct {
+      unsigned list_key[kSmList], list_token[kSmList];
+      unsigned long long short_mass[kSmShort];
+    };
+  };
   unsigned long long warp_mass[kSmCluster * kSmWarps];  // every warp of the cluster
   unsigned warp_ties[kSmCluster * kSmWarps];
   unsigned long long seg_mass[kSmCluster];  // of every CTA's bins
   unsigned seg_cnt[kSmCluster];
-  unsigned long long top[kSmCluster];  // (ordered value, inverted index) of every CTA's maximum
+  unsigned long long warp_top[kSmCluster * kSmWarps];  // (ordered value, inverted index) of every warp's maximum
   unsigned long long scan_mass[kSmWarps];
   unsigned scan_cnt[kSmWarps];
   SampleBorder border;
+};
+
+// For a list that is not short, in the row's place once the list is made.
+struct SampleLong {
+  unsigned cnt[kSmBins], lo[kSmBins], hi[kSmBins];
+  unsigned long long mass[kSmShort];  // of the border bin's tokens
+  unsigned key[kSmShort], place[kSmShort];
+  unsigned members, cut_key, cut_place;
+  unsigned long long cut_mass;  // up to the cut, its token included
 };
 
 // Values as unsigned numbers in the same order; -0 counts as 0, and what cannot
@@ -118,7 +140,8 @@ template <>
 __device__ __forceinline__ float sample_lowest<float>() { return -INFINITY; }
 
 __host__ inline size_t sample_smem_bytes(int slice, int item) {
-  return sizeof(SampleShared) + 16 + (size_t)slice * item;
+  const size_t row = (size_t)slice * item;
+  return sizeof(SampleShared) + 16 + (row > sizeof(SampleLong) ? row : sizeof(SampleLong));
 }
 
 template <typename T>
@@ -131,46 +154,72 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int base = rank * a.slice;                           // first token of this CTA
   const int seg = a.slice / kSmWarps;                        // tokens of a warp, a multiple of 8
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory");
   pdl_wait();
   pdl_trigger();
 
-  // ---- the row's slice into shared memory (filled up with -inf), and its maximum
-  const T* src = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.vocab + base;
-  const int live = max(0, min(a.slice, a.vocab - base));
-  constexpr int kPer = 16 / sizeof(T);
-  const int vec = (reinterpret_cast<uintptr_t>(src) & 15) == 0 ? live / kPer : 0;
-  for (int i = threadIdx.x; i < vec; i += kSmThreads) reinterpret_cast<uint4*>(xs)[i] = __ldcs(reinterpret_cast<const uint4*>(src) + i);
-  for (int i = vec * kPer + threadIdx.x; i < a.slice; i += kSmThreads) xs[i] = i < live ? src[i] : sample_lowest<T>();
-  __syncthreads();
-
-  auto each = [&](auto&& f) {  // f(tokens 8 lane .. + 7 of the warp's next 256, the first one's place in the slice)
+  // A warp owns a stretch of the tokens, a lane 8 of each 256 of it.
+  auto each = [&](auto&& f) {  // f(tokens i .. i + 7 of the slice, i)
     for (int i = warp * seg + 8 * lane; i < (warp + 1) * seg; i += 256) {
       float x[8];
       sample_load8<T>(xs + i, x);
       f(x, i);
     }
   };
-  unsigned long long best = 0ull;
-  each([&](const float (&x)[8], int i) {
+
+  // ---- the row's slice into shared memory (filled up with -inf), and the largest token of every lane and warp
+  const T* src = reinterpret_cast<const T*>(a.logits) + (size_t)row * a.vocab + base;
+  const int live = max(0, min(a.slice, a.vocab - base));
+  const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
+  float mine = -INFINITY;
+  int mine_at = 0;  // of its first place, the eight tokens it is among
+#pragma unroll 4
+  for (int i = warp * seg + 8 * lane; i < (warp + 1) * seg; i += 256) {
+    alignas(16) T v[8];
+    if (aligned && i + 8 <= live) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const unsigned long long k = ((unsigned long long)sample_key(x[j]) << 32) | (unsigned)~(unsigned)(base + i + j);
-      best = k > best ? k : best;
+      for (int j = 0; j < (int)sizeof(T) / 2; ++j)
+        reinterpret_cast<uint4*>(v)[j] = __ldcs(reinterpret_cast<const uint4*>(src + i) + j);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = i + j < live ? src[i + j] : sample_lowest<T>();
     }
-  });
+#pragma unroll
+    for (int j = 0; j < (int)sizeof(T) / 2; ++j) reinterpret_cast<uint4*>(xs + i)[j] = reinterpret_cast<uint4*>(v)[j];
+    float m = (float)v[0];
+#pragma unroll
+    for (int j = 1; j < 8; ++j) m = fmaxf(m, (float)v[j]);  // drops NaN
+    if (m > mine) {
+      mine = m;
+      mine_at = i;
+    }
+  }
+  unsigned long long best = 0ull;
+  if (mine > -INFINITY) {
+    while (!((float)xs[mine_at] == mine)) ++mine_at;
+    best = ((unsigned long long)sample_key(mine) << 32) | (unsigned)~(unsigned)(base + mine_at);
+  }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
     const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
     best = other > best ? other : best;
   }
-  if (lane == 0) sh.scan_mass[warp] = best;
-  __syncthreads();
-  if (threadIdx.x < C) {
-    for (int w = 0; w < kSmWarps; ++w) best = sh.scan_mass[w] > best ? sh.scan_mass[w] : best;
-    st_cluster_u64(cluster_addr(&sh.top[rank], threadIdx.x), best);
-  }
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");  // every CTA runs: its memory may be written
+  if (lane < C) st_cluster_u64(cluster_addr(&sh.warp_top[rank * kSmWarps + warp], lane), best);
   cluster_sync_all();
-  for (int c = 0; c < C; ++c) best = sh.top[c] > best ? sh.top[c] : best;
+  constexpr int kTops = C * kSmWarps / 32;
+  unsigned long long tops[kTops];  // a lane's share of the warps' largest
+  best = 0ull;
+#pragma unroll
+  for (int j = 0; j < kTops; ++j) {
+    tops[j] = sh.warp_top[lane + 32 * j];
+    best = tops[j] > best ? tops[j] : best;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    const unsigned long long other = __shfl_xor_sync(0xffffffffu, best, o);
+    best = other > best ? other : best;
+  }
   const unsigned top_key = (unsigned)(best >> 32);
   const float top = sample_value(top_key);
 
@@ -187,14 +236,13 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
   const float min_p = fminf(a.min_p ? a.min_p[row] : a.min_p_all, 1.f);
   const float inv_t = fminf(1.f / temperature, 3.402823466e38f);
 
-  // (max - x) / T, correctly rounded but for rare last bits; weights of it.
-  auto depth = [&](float x) {
-    if (x == top) return 0.f;
-    const float d = fminf(top - x, 3.402823466e38f);
-    const float y = d * inv_t;
-    return y < 128.f ? fmaf(fmaf(-y, temperature, d), inv_t, y) : y;
+  // (max - x) / T for the bins (0 at the maximum, infinite ones too), and the weight, of the same corrected to a
+  // rounding or two of 2^-24: its error would be the weight's.
+  auto depth = [&](float x) { return x == top ? 0.f : fminf(top - x, 3.402823466e38f) * inv_t; };
+  auto weight = [&](float x, float y) {
+    if (y < 128.f) y = fmaf(fmaf(-y, temperature, x == top ? 0.f : top - x), inv_t, y);
+    return expf(-y);
   };
-  auto weight = [&](float y) { return expf(-y); };
   auto mass_of = [](float w) { return (unsigned long long)__float2ull_rn(w * kSmOne); };
   auto bin_of = [](float y) { return (int)fminf(y * kSmBinsPerUnit, (float)(kSmBins - 1)); };
   auto sub_of = [](float y, int bin) {
@@ -204,6 +252,14 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
 
   const bool by_mass = top_p < 1.f;
 
+  auto every_token = [&](auto&& f) {
+    each([&](const float (&x)[8], int) {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) f(x[j]);
+    });
+  };
+  auto lane_tops = [&](auto&& f) { f(mine); };
+
   // Tokens of the cluster counted (and weighed) in `bins` slots: member(x, y,
   // slot) says whether a token counts, and where. Thread i < bins / 8 comes back
   // with slot rank * bins / 8 + i: its sums over the cluster and what lies before.
@@ -212,7 +268,7 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     unsigned count, before_count, key_or, key_and;
   };
   unsigned long long all_mass = 0ull;  // of the last histogram
-  auto histogram = [&](int bins, bool keys, auto&& member) {
+  auto histogram = [&](int bins, bool masses, bool keys, auto&& tokens, auto&& member) {
     __syncthreads();  // everyone has read the last border
     for (int i = threadIdx.x; i < bins; i += kSmThreads) {
       sh.cnt[i] = sh.lo[i] = sh.hi[i] = 0u;
@@ -223,38 +279,23 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     }
     if (threadIdx.x == 0) sh.border.found = 0u;
     __syncthreads();
-    each([&](const float (&x)[8], int) {
-      int at = -1;
-      unsigned n = 0;
-      unsigned long long q = 0ull;
-      auto flush = [&] {
-        if (at < 0) return;
-        atomicAdd(&sh.cnt[at], n);
+    tokens([&](float x) {
+      int slot;
+      if (!(x > -INFINITY)) return;
+      const float y = depth(x);
+      if (!member(x, y, slot)) return;
+      atomicAdd(&sh.cnt[slot], 1u);
+      if (masses) {
+        const unsigned long long q = mass_of(weight(x, y));
         const unsigned ql = (unsigned)q;
         unsigned qh = (unsigned)(q >> 32);
-        if (ql != 0u) qh += atomicAdd(&sh.lo[at], ql) + ql < ql;  // the carry
-        if (qh != 0u) atomicAdd(&sh.hi[at], qh);
-      };
-#pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (!(x[j] > -INFINITY)) continue;
-        const float y = depth(x[j]);
-        int slot;
-        if (!member(x[j], y, slot)) continue;
-        if (slot != at) {  // equal neighbours add up first
-          flush();
-          at = slot;
-          n = 0;
-          q = 0ull;
-        }
-        ++n;
-        if (by_mass) q += mass_of(weight(y));
-        if (keys) {
-          atomicOr(&sh.kor[slot], sample_key(x[j]));
-          atomicAnd(&sh.kand[slot], sample_key(x[j]));
-        }
+        if (ql != 0u) qh += atomicAdd(&sh.lo[slot], ql) + ql < ql;  // the carry
+        if (qh != 0u) atomicAdd(&sh.hi[slot], qh);
       }
-      flush();
+      if (keys) {
+        atomicOr(&sh.kor[slot], sample_key(x));
+        atomicAnd(&sh.kand[slot], sample_key(x));
+      }
     });
     cluster_sync_all();
     const int share = bins / C, i = rank * share + threadIdx.x;
@@ -336,6 +377,26 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     return sh.border;
   };
 
+  // The drawn token is the first at which the running mass exceeds this.
+  auto target_of = [&](unsigned long long total) {
+    const double u = (double)a.uniforms[row];
+    const unsigned long long t = u > 0.0 ? (unsigned long long)(fmin(u, 1.0) * (double)total) : 0ull;
+    return t >= total ? total - 1ull : t;  // the maximum's own weight keeps total above 0
+  };
+
+  constexpr int kLowBits = 32 - 8 * (int)sizeof(T);  // bits of the pattern that a bf16 does not have
+  // Sum over the warp of masses below 2^59, in three parts whose sums fit 32 bits.
+  auto warp_sum64 = [](unsigned long long v) {
+    const unsigned long long s0 = __reduce_add_sync(0xffffffffu, (unsigned)(v & 0x3fffffu));
+    const unsigned long long s1 = __reduce_add_sync(0xffffffffu, (unsigned)(v >> 22 & 0x3fffffu));
+    const unsigned long long s2 = __reduce_add_sync(0xffffffffu, (unsigned)(v >> 44));
+    return s0 + (s1 << 22) + (s2 << 44);
+  };
+  // Mass that top-p keeps of `whole`: ranks before which less than it lies.
+  auto wanted = [&](unsigned long long whole) {
+    return max(1ull, (unsigned long long)ceil((double)fmaxf(top_p, 0.f) * (double)whole));
+  };
+
   // What is kept: tokens of a bin before bin1, and of bin1 (unless all of it) of
   // a sub-bin before bin2, and of bin2 (unless all of it) those above `key` and
   // the first `ties` of those equal to it.
@@ -352,7 +413,7 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     unsigned need = count - b1.before_count;
     unsigned long long need_mass = mass - b1.before_mass;
     const int want1 = bin1;
-    SampleBorder b = search(histogram(kSmBins, true, [&](float, float y, int& slot) {
+    SampleBorder b = search(histogram(kSmBins, by_mass, true, every_token, [&](float, float y, int& slot) {
                               if (bin_of(y) != want1) return false;
                               slot = sub_of(y, want1);
                               return true;
@@ -365,7 +426,7 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
       const int want2 = bin2;
       unsigned head = 0u;
       for (int shift = 24; shift >= 0; shift -= 8) {
-        b = search(histogram(256, true, [&](float x, float y, int& slot) {
+        b = search(histogram(256, by_mass, true, every_token, [&](float x, float y, int& slot) {
                      const unsigned k = sample_key(x);
                      if (bin_of(y) != want1 || sub_of(y, want1) != want2 || (shift < 24 && k >> (shift + 8) != head))
                        return false;
@@ -383,23 +444,408 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     ties = mass_wanted ? (unsigned)min((unsigned long long)b.count, one > 0ull ? (need_mass + one - 1ull) / one : 1ull) : need;
     kept_mass += one * ties;
   };
+  // The tokens at or above `least` and in the bins up to `last`, if they are few
+  // enough: put in a list in index order, and the rest is up to the first CTA.
+  // They have to be a first stretch of the ranks that holds all that is kept;
+  // whole: the mass that top-p refers to, 0 for that of the list after top-k.
+  auto finish_in_list = [&](float least, int last, bool cut_count, unsigned long long whole) {
+    auto in = [&](float x) { return x >= least && x > -INFINITY && (last >= kSmBins || bin_of(depth(x)) <= last); };
+    const bool some = __any_sync(0xffffffffu, in(mine));  // most warps have none
+    unsigned n = 0;
+    if (some)
+      each([&](const float (&x)[8], int) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) n += in(x[j]);
+      });
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (lane < C) st_cluster_u32(cluster_addr(&sh.warp_ties[rank * kSmWarps + warp], lane), n);
+    cluster_sync_all();
+    unsigned at = 0, all = 0;
+    for (int w = lane; w < C * kSmWarps; w += 32) {
+      const unsigned v = sh.warp_ties[w];
+      all += v;
+      if (w < rank * kSmWarps + warp) at += v;
+    }
+    at = __reduce_add_sync(0xffffffffu, at);
+    all = __reduce_add_sync(0xffffffffu, all);
+    if (all > kSmList) {
+      cluster_sync_all();  // the counts are read before they are written again
+      return false;
+    }
+    if (n > 0)
+      for (int i0 = warp * seg; i0 < (warp + 1) * seg; i0 += 256) {
+        const int i = i0 + 8 * lane;
+        float x[8];
+        unsigned is = 0u;
+        if (i < (warp + 1) * seg) {
+          sample_load8<T>(xs + i, x);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) is |= in(x[j]) ? 1u << j : 0u;
+        }
+        if (!__any_sync(0xffffffffu, is != 0u)) continue;
+        unsigned upto = __popc(is);
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+          const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+          if (lane >= o) upto += v;
+        }
+        for (unsigned p = at + upto - __popc(is); is != 0u; is &= is - 1u, ++p) {
+          const int j = __ffs(is) - 1;
+          st_cluster_u32(cluster_addr(&sh.list_key[p], 0), sample_key((float)xs[i + j]));
+          st_cluster_u32(cluster_addr(&sh.list_token[p], 0), (unsigned)(base + i + j));
+        }
+        at += __shfl_sync(0xffffffffu, upto, 31);
+      }
+    cluster_sync_all();  // the last access to another CTA's memory is before it
+    if (rank != 0) return true;
+    if (all <= kSmShort) {
+      // Short: a thread a token counts what ranks ahead of it. (The bit-by-bit search below takes two dozen barriers.)
+      const unsigned p = threadIdx.x;
+      unsigned k = 0u, ahead = 0u;
+      unsigned long long q = 0ull, ahead_mass = 0ull;
+      float w = 0.f;
+      if (p < all) {
+        k = sh.list_key[p];
+        w = weight(sample_value(k), depth(sample_value(k)));
+        q = mass_of(w);
+        sh.short_mass[p] = q;
+      }
+      __syncthreads();
+      if (p < all)
+#pragma unroll 4
+        for (unsigned j = 0; j < all; ++j) {
+          const unsigned o = sh.list_key[j];
+          if (o > k || (o == k && j < p)) {
+            ++ahead;
+            ahead_mass += sh.short_mass[j];
+          }
+        }
+      const bool counted = p < all && (!cut_count || ahead < (unsigned)top_k);
+      if (by_mass) {
+        if (whole == 0ull) {  // of what top-k has left: known to its last rank
+          if (p < all && ahead == min(cut_count ? (unsigned)top_k : all, all) - 1u) sh.seg_mass[0] = ahead_mass + q;
+          __syncthreads();
+          whole = sh.seg_mass[0];
+        }
+      }
+      if (!counted || (by_mass && ahead_mass >= wanted(whole)) || !(w >= min_p)) q = 0ull;
+      unsigned long long upto = q;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned long long v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) sh.scan_mass[warp] = upto;
+      __syncthreads();
+      unsigned long long before = upto - q, total = 0ull;
+#pragma unroll
+      for (int v = 0; v < kSmShort / 32; ++v) {
+        if (v < warp) before += sh.scan_mass[v];
+        total += sh.scan_mass[v];
+      }
+      const unsigned long long target = target_of(total);
+      if (target >= before && target < before + q) a.out[row] = sh.list_token[p];
+      return true;
+    }
+    constexpr int kEach = kSmList / kSmThreads;
+    unsigned key_of[kEach];
+    unsigned long long mass[kEach];
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      const unsigned p = threadIdx.x * kEach + j;
+      key_of[j] = p < all ? sh.list_key[p] : 0u;
+      mass[j] = 0ull;
+      if (p < all) {
+        const float x = sample_value(key_of[j]);
+        mass[j] = mass_of(weight(x, depth(x)));
+      }
+    }
+    int turn = 0;
+    // Count or mass over the list: two buffers, so that one barrier a call is enough.
+    auto block_sum = [&](unsigned long long v) {
+      v = warp_sum64(v);
+      unsigned long long* buf = sh.warp_mass + 32 * (turn++ & 1);
+      if (lane == 0) buf[warp] = v;
+      __syncthreads();
+      unsigned long long t = 0ull;
+#pragma unroll
+      for (int w = 0; w < kSmWarps; ++w) t += buf[w];
+      return t;
+    };
+    auto over = [&](unsigned least, bool weigh) {  // tokens at or above it
+      unsigned long long v = 0ull;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) v += key_of[j] >= least ? (weigh ? mass[j] : 1ull) : 0ull;
+      return v;
+    };
+    // Of the tokens kept so far, those behind the rank whose count or mass reaches `want` go. Bit by bit, each with a
+    // barrier: for many (nearly) equal tokens.
+    auto cut = [&](bool weigh, unsigned long long want) {
+      unsigned border = 0u;
+      for (int bit = 31; bit >= kLowBits; --bit) {
+        const unsigned c = border | 1u << bit;
+        if (block_sum(over(c, weigh)) >= want) border = c;
+      }
+      const unsigned above = border + (1u << kLowBits);  // 0 only past the largest pattern, which no value has
+      const unsigned long long rest = want - block_sum(over(above, weigh));
+      unsigned eq = 0;
+      unsigned long long one = 0ull;
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (key_of[j] >= border && key_of[j] < above) {
+          ++eq;
+          one = mass[j];
+        }
+      // equal tokens in index order: those of the threads before, then this one's
+      unsigned upto = eq;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      if (lane == 31) sh.scan_cnt[warp] = upto;
+      __syncthreads();
+      unsigned r = upto - eq;
+      for (int w = 0; w < warp; ++w) r += sh.scan_cnt[w];
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j) {
+        bool keep = key_of[j] >= above;
+        if (key_of[j] >= border && key_of[j] < above) {
+          keep = weigh ? r * one < rest : r < rest;
+          ++r;
+        }
+        if (!keep) {
+          mass[j] = 0ull;
+          key_of[j] = 0u;
+        }
+      }
+    };
+    // The list in bins of equal width in (max - x) / T, counted and weighed; a thread has two of them.
+    SampleLong& big = *reinterpret_cast<SampleLong*>(xs);
+    const float per_unit = (kSmBins - 1) / fmaxf(least > -INFINITY ? depth(least) : (float)(last + 1) / kSmBinsPerUnit, 1e-20f);
+    auto slot_of = [&](unsigned k) { return (int)fminf(depth(sample_value(k)) * per_unit, (float)(kSmBins - 1)); };
+    for (int i = threadIdx.x; i < kSmBins; i += kSmThreads) big.cnt[i] = big.lo[i] = big.hi[i] = 0u;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kEach; ++j)
+      if (key_of[j] != 0u) {
+        const int i = slot_of(key_of[j]);
+        atomicAdd(&big.cnt[i], 1u);
+        const unsigned l = (unsigned)mass[j];
+        const unsigned h = (unsigned)(mass[j] >> 32) + (l != 0u && atomicAdd(&big.lo[i], l) + l < l);
+        if (h != 0u) atomicAdd(&big.hi[i], h);
+      }
+    __syncthreads();
+    unsigned bin_n[2];
+    unsigned long long bin_q[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int i = 2 * threadIdx.x + h;
+      bin_n[h] = big.cnt[i];
+      bin_q[h] = ((unsigned long long)big.hi[i] << 32) + big.lo[i];
+    }
+    unsigned n_upto = bin_n[0] + bin_n[1];
+    unsigned long long q_upto = bin_q[0] + bin_q[1];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned un = __shfl_up_sync(0xffffffffu, n_upto, o);
+      const unsigned long long uq = __shfl_up_sync(0xffffffffu, q_upto, o);
+      if (lane >= o) {
+        n_upto += un;
+        q_upto += uq;
+      }
+    }
+    if (lane == 31) {
+      sh.scan_cnt[warp] = n_upto;
+      sh.scan_mass[warp] = q_upto;
+    }
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) {
+      n_upto += sh.scan_cnt[w];
+      q_upto += sh.scan_mass[w];
+    }
+    // As cut(), by the bins: the border's bin, and in it, where it is short, token by token. Gives the mass up to the cut.
+    auto cut_by_bins = [&](bool weigh, unsigned long long want) {
+      unsigned n = n_upto - bin_n[0] - bin_n[1];
+      unsigned long long q = q_upto - bin_q[0] - bin_q[1];
+      if (threadIdx.x == 0) {
+        sh.border.found = 0u;
+        big.members = 0u;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        if (weigh ? q < want && q + bin_q[h] >= want : n < want && n + bin_n[h] >= want) {
+          sh.border.before_count = n;
+          sh.border.before_mass = q;
+          sh.border.count = bin_n[h];
+          sh.border.slot = 2 * threadIdx.x + h;
+          sh.border.found = 1u;
+        }
+        n += bin_n[h];
+        q += bin_q[h];
+      }
+      __syncthreads();
+      const SampleBorder b = sh.border;
+      if (!b.found) return 0ull;  // nothing to cut
+      if (b.count > kSmShort) {
+        cut(weigh, want);
+        unsigned long long v = 0ull;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) v += mass[j];
+        return block_sum(v);
+      }
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (key_of[j] != 0u && slot_of(key_of[j]) == (int)b.slot) {
+          const unsigned p = atomicAdd(&big.members, 1u);
+          big.key[p] = key_of[j];
+          big.place[p] = threadIdx.x * kEach + j;
+          big.mass[p] = mass[j];
+        }
+      __syncthreads();
+      const unsigned members = big.members;
+      if (threadIdx.x < members) {
+        const unsigned k = big.key[threadIdx.x], place = big.place[threadIdx.x];
+        const unsigned long long m = big.mass[threadIdx.x];
+        unsigned long long count = b.before_count, ahead = b.before_mass;
+#pragma unroll 4
+        for (unsigned j = 0; j < members; ++j) {
+          const unsigned o = big.key[j];
+          if (o > k || (o == k && big.place[j] < place)) {
+            ++count;
+            ahead += big.mass[j];
+          }
+        }
+        // the last kept rank: what lies before it is below the wanted, what lies up to it is not
+        if (weigh ? ahead < want && ahead + m >= want : count + 1ull == want) {
+          big.cut_key = k;
+          big.cut_place = place;
+          big.cut_mass = ahead + m;
+        }
+      }
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kEach; ++j)
+        if (key_of[j] < big.cut_key || (key_of[j] == big.cut_key && threadIdx.x * kEach + j > big.cut_place)) {
+          key_of[j] = 0u;
+          mass[j] = 0ull;
+        }
+      return big.cut_mass;
+    };
+    if (cut_count) {
+      const unsigned long long v = cut_by_bins(false, (unsigned long long)top_k);
+      if (whole == 0ull) whole = v;
+    }
+    if (by_mass) {
+      if (whole == 0ull) {  // of the list
+        unsigned long long v = 0ull;
+#pragma unroll
+        for (int j = 0; j < kEach; ++j) v += mass[j];
+        whole = block_sum(v);
+      }
+      cut_by_bins(true, wanted(whole));
+    }
+    unsigned long long v = 0ull;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      if (key_of[j] != 0u) {
+        const float x = sample_value(key_of[j]);
+        if (!(weight(x, depth(x)) >= min_p)) mass[j] = 0ull;
+      }
+      v += mass[j];
+    }
+    unsigned long long upto = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const unsigned long long w = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += w;
+    }
+    if (lane == 31) sh.scan_mass[warp] = upto;
+    __syncthreads();
+    unsigned long long before = upto - v, total = 0ull;
+    for (int w = 0; w < kSmWarps; ++w) {
+      if (w < warp) before += sh.scan_mass[w];
+      total += sh.scan_mass[w];
+    }
+    const unsigned long long target = target_of(total);
+    if (target < before || target >= before + v) return true;
+    int pick = -1;
+#pragma unroll
+    for (int j = 0; j < kEach; ++j) {
+      before += mass[j];
+      if (pick < 0 && before > target) pick = j;
+    }
+    a.out[row] = sh.list_token[threadIdx.x * kEach + pick];
+    return true;
+  };
+
   if (top_k > 0 || by_mass) {
-    const Slot s = histogram(kSmBins, false, [&](float, float y, int& slot) {
+    auto all_bins = [&](float, float y, int& slot) {
       slot = bin_of(y);
       return true;
-    });
+    };
+    SampleBorder b;
+    unsigned long long whole = 0ull;  // mass of all tokens: what top-p refers to without top-k
+    if (top_k <= 0) {
+      double sum = 0.0;  // integers below 2^53: exact
+      every_token([&](float x) {
+        if (x > -INFINITY) sum += (double)rintf(weight(x, depth(x)) * kSmOne);
+      });
+      unsigned long long q = (unsigned long long)sum;
+      q = warp_sum64(q);
+      if (lane < C) st_cluster_u64(cluster_addr(&sh.warp_mass[rank * kSmWarps + warp], lane), q);
+      cluster_sync_all();
+      for (int w = lane; w < C * kSmWarps; w += 32) whole += sh.warp_mass[w];
+      whole = warp_sum64(whole);
+    }
+    // A cheap first stretch of the ranks: as many warps' maxima as top_k asks
+    // for, or of the mass that top_p asks for, are that many tokens, so
+    // everything ranked after them all is dropped. Then the same with the lanes' maxima.
+    if (a.vocab <= kSmShort) {
+      finish_in_list(-INFINITY, kSmBins, top_k > 0 && top_k < a.vocab, whole);
+      return;
+    }
+    const unsigned long long want = top_k > 0 ? 0ull : wanted(whole);
+    if (top_k <= kSmWarps * C / 2) {
+      unsigned long long weigh[kTops];
+#pragma unroll
+      for (int j = 0; j < kTops; ++j) {
+        const float x = sample_value((unsigned)(tops[j] >> 32));
+        weigh[j] = top_k > 0 ? 1ull : tops[j] != 0ull ? mass_of(weight(x, depth(x))) : 0ull;
+      }
+      const unsigned long long wish = top_k > 0 ? (unsigned long long)top_k : want;
+      auto over = [&](unsigned c) {  // count or mass of the maxima whose pattern is at least c
+        unsigned long long v = 0ull;
+#pragma unroll
+        for (int j = 0; j < kTops; ++j) v += (unsigned)(tops[j] >> 32) >= c ? weigh[j] : 0ull;
+        return top_k > 0 ? (unsigned long long)__reduce_add_sync(0xffffffffu, (unsigned)v) : warp_sum64(v);
+      };
+      unsigned border = 0u;
+      for (int bit = 31; bit >= kLowBits; --bit)
+        if (over(border | 1u << bit) >= wish) border |= 1u << bit;
+      // every value at or above the border's pattern (its low bits lack where bf16 has none: not above the value)
+      if (border != 0u && finish_in_list(sample_value(border), kSmBins, top_k > 0, whole)) return;
+    }
+    if (top_k <= kSmList) {
+      b = search(histogram(kSmBins, top_k <= 0, false, lane_tops, all_bins), kSmBins, top_k <= 0, (unsigned)top_k, want);
+      if (b.found && finish_in_list(-INFINITY, (int)b.slot, top_k > 0, whole)) return;
+    }
+    const Slot s = histogram(kSmBins, by_mass, false, every_token, all_bins);
     kept_mass = all_mass;
     if (top_k > 0) {
-      const SampleBorder b = search(s, kSmBins, false, (unsigned)top_k, 0ull);
+      b = search(s, kSmBins, false, (unsigned)top_k, 0ull);
       if (b.found) refine(b, false, (unsigned)top_k, 0ull);
     }
     if (by_mass) {
-      const unsigned long long want = max(1ull, (unsigned long long)ceil((double)fmaxf(top_p, 0.f) * (double)kept_mass));
+      const unsigned long long mass = wanted(kept_mass);
       __syncthreads();
       if (threadIdx.x == 0) sh.border.found = 0u;
       cluster_sync_all();
-      const SampleBorder b = search(s, kSmBins, true, 0u, want);
-      if (b.found) refine(b, true, 0u, want);
+      b = search(s, kSmBins, true, 0u, mass);
+      if (b.found && finish_in_list(-INFINITY, (int)b.slot, false, kept_mass)) return;
+      if (b.found) refine(b, true, 0u, mass);
     }
   }
 
@@ -422,7 +868,7 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
         const float y = depth(x[j]);
-        n += state_of(x[j], y, weight(y)) == 2;
+        n += state_of(x[j], y, weight(x[j], y)) == 2;
       }
     });
     n = __reduce_add_sync(0xffffffffu, n);
@@ -443,7 +889,7 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
         sample_load8<T>(xs + i, x);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const float y = depth(x[j]), w = weight(y);
+          const float y = depth(x[j]), w = weight(x[j], y);
           const int st = state_of(x[j], y, w);
           q[j] = st != 0 ? mass_of(w) : 0ull;
           tie |= st == 2 ? 1u << j : 0u;
@@ -493,9 +939,7 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     total += __shfl_xor_sync(0xffffffffu, total, o);
     before += __shfl_xor_sync(0xffffffffu, before, o);
   }
-  const double u = (double)a.uniforms[row];
-  unsigned long long target = u > 0.0 ? (unsigned long long)(fmin(u, 1.0) * (double)total) : 0ull;
-  if (target >= total) target = total - 1ull;  // the maximum's own weight keeps total above 0
+  const unsigned long long target = target_of(total);
   if (target < before || target >= before + sum) return;
   kept([&](const unsigned long long (&q)[8], int i) {
     unsigned long long m = 0ull;

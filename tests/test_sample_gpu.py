@@ -69,7 +69,8 @@ def check(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0):
 SETTINGS = [dict(), dict(top_k=1), dict(top_k=20), dict(top_k=3000), dict(top_p=0.9), dict(top_p=0.05), dict(min_p=0.05),
             dict(temperature=0.6, top_k=20, top_p=0.95), dict(temperature=1.7, top_k=500, top_p=0.5, min_p=0.01),
             dict(temperature=0.0), dict(temperature=0.01), dict(temperature=50.0, top_p=0.7), dict(top_k=2 ** 31 - 1),
-            dict(top_p=1e-6), dict(min_p=1.0)]
+            dict(top_p=1e-6), dict(min_p=1.0), dict(top_k=64), dict(top_k=65, top_p=0.7), dict(top_k=2500, top_p=0.99),
+            dict(top_k=4097), dict(top_k=200, top_p=0.97, min_p=0.02), dict(temperature=1.2, top_p=0.999), dict(temperature=3.0, top_p=0.4)]
 
 
 @pytest.mark.parametrize("vocab", [1, 7, 100, 4096, 50257, 151936, 262144])
