@@ -22,13 +22,10 @@
 //  * warps 4-7 and 8-11: softmax of M tile 0 and 1, a thread per row. The
 //    reference maximum only moves when a row's maximum grows by more than 8 (P
 //    stays below 2^8 and keeps its relative precision), so O is seldom rescaled.
-//  * warp 2, one lane: walks the CTA's pieces of units ahead of the others and
-//    hands them over through a ring of 4 (the lookups and divisions of a new
-//    piece took 3 us of every role's time when each made them itself).
-// The register file is split by setmaxnreg: 384 threads start with 168 each
-// (64512); the first warpgroup keeps 104 (fewer spill: its roles' spills go to L2, as
-// shared memory leaves next to no L1), the softmax groups take 200:
-// 128 * 104 + 256 * 200 = 64512.
+//  * warp 2: walks the CTA's pieces of units ahead of the others and hands them
+//    over through a ring of 4 (the lookups and divisions of a new piece took 3 us
+//    of every role's time when each made them itself); and waits for K and V on
+//    the MMA warps' behalf.
 // Every wait is bounded; on failure an error is recorded, the roles stop, and
 // TMEM is released after the MMAs that were issued.
 #pragma once
@@ -43,7 +40,7 @@ constexpr int kPtThreads = 12 * 32;
 constexpr int kPtTile = 128 * 128 * 2;         // a Q tile: 32 KB, dims 0-63 then 64-127
 constexpr int kPtKvTile = kPtKeys * 128 * 2;   // a K or V tile: 16 KB, likewise
 constexpr int kPtSlots = 4;                    // ring slots of each
-constexpr int kPtMaxUnits = 7168;
+constexpr int kPtMaxUnits = 4096;
 constexpr int kPtMinTiles = 2;
 
 constexpr int kPtPieces = 4;
@@ -74,7 +71,7 @@ struct PagedTcArgs {
 };
 
 __host__ inline size_t pt_smem_bytes(int max_units) {
-  return 1024 + 2 * (size_t)kPtTile + 2 * kPtSlots * (size_t)kPtKvTile + 512 + kPtPieces * sizeof(PtPiece) + (size_t)(kPagedMaxSeqs + 1 + max_units + 1) * 4;
+  return 1024 + 2 * (size_t)kPtTile + 2 * kPtSlots * (size_t)kPtKvTile + 512 + kPtPieces * sizeof(PtPiece) + (size_t)(4 * kPagedMaxSeqs + 1 + max_units + 1) * 4;
 }
 
 // The MMAs as the whole warp runs them: `lead` (one lane) issues. Kept free of
@@ -194,14 +191,15 @@ struct TcUnit {
   int seq, token0, tokens, p_first, kv, hi;  // p_first: position of token0; hi: one past the last key a row sees
   TileSpan ts;
 };
-__device__ __forceinline__ TcUnit tc_unit(const PagedBatch& b, const int* seq_unit, int u, int per_unit) {
+__device__ __forceinline__ TcUnit tc_unit(const PagedBatch& b, const SeqSpan* seqs, const int* seq_unit, int u,
+                                          int per_unit) {
   int lo = 0, hi = b.n_seqs - 1;
   while (lo < hi) {  // the sequence of unit u: the first with seq_unit[seq + 1] > u
     const int mid = (lo + hi) >> 1;
     if (seq_unit[mid + 1] > u) hi = mid;
     else lo = mid + 1;
   }
-  const SeqSpan sp = paged_seq(b, lo, nullptr);
+  const SeqSpan sp = seqs[lo];
   TcUnit r;
   r.seq = lo;
   const int i0 = (u - seq_unit[lo]) * per_unit;
@@ -262,7 +260,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   volatile int* flags = reinterpret_cast<volatile int*>(tmem_slot + 1);
   int* warp_tot = reinterpret_cast<int*>(tmem_slot + 2);  // [12]
   PtPiece* pieces = reinterpret_cast<PtPiece*>(bars + 64);
-  int* seq_unit = reinterpret_cast<int*>(pieces + kPtPieces);  // [n_seqs + 1] units before each sequence
+  SeqSpan* seqs = reinterpret_cast<SeqSpan*>(pieces + kPtPieces);
+  int* seq_unit = reinterpret_cast<int*>(seqs + kPagedMaxSeqs);  // [n_seqs + 1] units before each sequence
   int* unit_tile = seq_unit + kPagedMaxSeqs + 1;          // [units + 1] tiles before each unit
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
@@ -278,14 +277,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       mbar_init(&q_empty[t], 1);
       for (int i = 2 * t; i < 2 * t + 2; ++i) {
         mbar_init(&s_full[i], 1);
-        mbar_init(&p_full[i], 4);
+        mbar_init(&p_full[i], 5);
         mbar_init(&o_done[i], 1);
       }
       mbar_init(&done[t], 1);
     }
     for (int i = 0; i < kPtPieces; ++i) {
       mbar_init(&piece_full[i], 1);
-      mbar_init(&piece_empty[i], 11);  // producer, 2 MMA warps, 8 softmax warps
+      mbar_init(&piece_empty[i], 12);  // producer, 2 MMA warps, warp 2, 8 softmax warps
     }
     fence_mbar_init();
     flags[0] = 0;
@@ -312,9 +311,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   int units = 0;
   for (int s0 = 0; s0 < b.n_seqs; s0 += kPtThreads) {
     const int s = s0 + threadIdx.x;
-    const int n = s < b.n_seqs ? paged_seq(b, s, a.err).n : 0;
-    const int v = block_scan((n + 2 * RH - 1) / (2 * RH), warp_tot, units);
-    if (s < b.n_seqs) seq_unit[s + 1] = v;
+    const SeqSpan sp = s < b.n_seqs ? paged_seq(b, s, a.err) : SeqSpan{0, 0, 0};
+    const int v = block_scan((sp.n + 2 * RH - 1) / (2 * RH), warp_tot, units);
+    if (s < b.n_seqs) {
+      seqs[s] = sp;
+      seq_unit[s + 1] = v;
+    }
   }
   __syncthreads();
   if (units > a.max_units) {  // sequences that overlap
@@ -324,7 +326,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   int tiles = 0;
   for (int u0 = 0; u0 < units; u0 += kPtThreads) {
     const int u = u0 + threadIdx.x;
-    const int v = block_scan(u < units ? tc_unit(b, seq_unit, u, 2 * RH).ts.count : 0, warp_tot, tiles);
+    const int v = block_scan(u < units ? tc_unit(b, seqs, seq_unit, u, 2 * RH).ts.count : 0, warp_tot, tiles);
     if (u < units) unit_tile[u + 1] = v;
   }
   __syncthreads();
@@ -418,30 +420,30 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         if (quse[t] > 0) mbar_wait(&q_full[t], (quse[t] - 1) & 1, nullptr, 0);
       for (int i = max(0, issued - kPtSlots); i < issued + (ok ? 0 : 1); ++i)
         for (int kv = 0; kv < 2; ++kv) mbar_wait(&kv_full[kv * kPtSlots + i % kPtSlots], (i / kPtSlots) & 1, nullptr, 0);
-    } else if (warp == 2 && lane == 0) {
-      // ------------------------------------------------------------- scheduler
+    } else if (warp == 2) {
+      // ----------------------------------------------- scheduler and gatekeeper
       int u = 0;
       for (int hi = max(0, units - 1); u < hi;) {  // the unit of tile t_begin
         const int mid = (u + hi) >> 1;
         if ((long long)unit_tile[mid + 1] * a.Hkv > t_begin) hi = mid;
         else u = mid + 1;
       }
-      long long t = t_begin;
+      long long at = t_begin, base = 0;
       TcUnit un;
-      int n = 0, fresh = -1;  // fresh: the unit `un` describes
-      long long base = 0;
-      for (int i = 0;; ++i) {
-        const int e = i % kPtPieces;
+      int n = 0, fresh = -1, made = 0;  // fresh: the unit that `un` describes
+      bool more = true, ok = true;
+      auto hand_over = [&] {  // the next piece into the ring
+        const int e = made % kPtPieces;
         PtPiece p;
         p.k0 = p.k1 = 0;  // the end of the CTA's work
-        if (t < t_end) {
+        if (at < t_end) {
           if (fresh != u) {
-            un = tc_unit(b, seq_unit, u, 2 * RH);
+            un = tc_unit(b, seqs, seq_unit, u, 2 * RH);
             n = unit_tile[u + 1] - unit_tile[u];
             base = (long long)unit_tile[u] * a.Hkv;
             fresh = u;
           }
-          const int g = (int)((t - base) / n);
+          const int g = (int)((at - base) / n);
           const long long u0 = base + (long long)g * n;
           p.seq = un.seq;
           p.token0 = un.token0;
@@ -452,19 +454,46 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           p.n_sink = un.ts.n_sink;
           p.lo = un.ts.lo;
           p.head = g;
-          p.k0 = (int)(t - u0);
-          p.k1 = (int)min((long long)n, p.k0 + (t_end - t));
+          p.k0 = (int)(at - u0);
+          p.k1 = (int)min((long long)n, p.k0 + (t_end - at));
           p.whole = p.k0 == 0 && p.k1 == n;
-          p.first = t == t_begin;
+          p.first = at == t_begin;
           p.last = p.k0 == 0 && !p.whole ? tile_owner(u0 + n - 1, total, E) : -1;
-          t += p.k1 - p.k0;
+          at += p.k1 - p.k0;
           if (g == a.Hkv - 1 && p.k1 == n) ++u;
         }
-        if (i >= kPtPieces && !mbar_wait(&piece_empty[e], ((i / kPtPieces) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY)) break;
-        pieces[e] = p;
-        mbar_arrive(&piece_full[e]);
-        if (p.k0 == p.k1 || flags[0] != 0) break;
-      }
+        if (made >= kPtPieces)
+          ok = __all_sync(0xffffffffu, mbar_wait(&piece_empty[e], ((made / kPtPieces) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY));
+        if (!ok) return;
+        if (lane == 0) {
+          pieces[e] = p;
+          mbar_arrive(&piece_full[e]);
+        }
+        ++made;
+        more = p.k0 != p.k1;
+      };
+      while (more && made < kPtPieces) hand_over();
+      // The gatekeeper waits for the K and V tiles that a step's MMAs read and
+      // joins P's barrier for them: the MMA warps' own waits took 280 cycles
+      // each even where nothing was to be waited for, a quarter of their time.
+      int J = 0;
+      uint32_t phase = 0;  // bit 2 t + buffer
+      walk([&](const PtPiece& pc) {
+        const int steps = pc.k1 - pc.k0, nt = pc.tokens > RH ? 2 : 1;
+        for (int k = 0; k < steps && ok; ++k, ++J) {
+          ok = mbar_wait(&kv_full[kPtSlots + J % kPtSlots], (J / kPtSlots) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          if (ok && k + 2 < steps) ok = mbar_wait(&kv_full[(J + 2) % kPtSlots], ((J + 2) / kPtSlots) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
+          for (int t = 0; t < nt && ok; ++t) {
+            const int i = 2 * t + (J & 1);
+            ok = mbar_wait(&p_full[i], ((phase >> i) & 1) ^ 1, a.err, DEV_TIMEOUT_ATTN_FULL);  // the tile before it is through
+            if (ok && lane == 0) mbar_arrive(&p_full[i]);
+            phase ^= 1u << i;
+          }
+          ok = __all_sync(0xffffffffu, ok);
+        }
+        if (ok && more) hand_over();
+        return ok && flags[0] == 0;
+      }, [] {});
     } else if (warp == 1 || warp == 3) {
       // ------------------------------------------------------------ MMA issuer
       const uint32_t idesc_s = pg_idesc(128, kPtKeys);
@@ -489,7 +518,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           J += n;
           return true;
         }
-        auto full = [&](int kv, int j) { return wait(&kv_full[kv * kPtSlots + j % kPtSlots], (j / kPtSlots) & 1); };
+        auto k_full = [&](int j) { return wait(&kv_full[j % kPtSlots], (j / kPtSlots) & 1); };
         // a slot is free after both M tiles' MMAs; of a lone tile it is released twice
         auto release = [&](int kv, int j) {
           tc_commit_by(lead, &kv_empty[kv * kPtSlots + j % kPtSlots]);
@@ -504,22 +533,21 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           tc_commit_by(lead, &s_full[2 * t + (j & 1)]);
           release(0, j);
         };
-        ok = wait(&q_full[t], qphase) && full(0, J);
+        ok = wait(&q_full[t], qphase) && k_full(J);
         if (!ok) return false;
         qphase ^= 1;
         tc_fence_after();
         issue_s(J);
         if (n > 1) {
-          ok = full(0, J + 1);
+          ok = k_full(J + 1);
           if (!ok) return false;
           tc_fence_after();
           issue_s(J + 1);
         }
         if (n <= 2) tc_commit_by(lead, &q_empty[t]);
-        ok = full(1, J) && (n <= 2 || full(0, J + 2));
 #pragma unroll 1
         for (int k = 0; k < n && ok; ++k, ++J) {
-          ok = wait(&p_full[2 * t + (J & 1)], (pphase >> (J & 1)) & 1);
+          ok = wait(&p_full[2 * t + (J & 1)], (pphase >> (J & 1)) & 1);  // P, and K and V (warp 2)
           if (!ok) break;
           pphase ^= 1 << (J & 1);
           tc_fence_after();
@@ -534,8 +562,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
             issue_s(J + 2);  // over P's buffer: runs after P . V, as issued
             if (k + 3 == n) tc_commit_by(lead, &q_empty[t]);
           }
-          // what the next pass needs, waited for under this one's MMAs
-          if (k + 1 < n) ok = full(1, J + 1) && (k + 3 >= n || full(0, J + 3));
         }
         return ok;
       }, [&] { ok = false; });

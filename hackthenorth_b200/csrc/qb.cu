@@ -75,10 +75,14 @@ int sm_count_of(int device) {
   return n;
 }
 
+// SMs of the current device; looked up once per device.
 int current_sm_count() {
+  static int known[64] = {};
   int dev = 0;
   cudaGetDevice(&dev);
-  return sm_count_of(dev);
+  if (dev < 0 || dev >= 64) return sm_count_of(dev);
+  if (known[dev] == 0) known[dev] = sm_count_of(dev);
+  return known[dev];
 }
 
 // Function attributes (cudaFuncSetAttribute) and occupancy results belong to

@@ -47,12 +47,14 @@ def _bf16_cuda(*ts):
 
 def check_device_errors(device=None) -> None:
     """Synchronise and raise if an op-level kernel reported a device error."""
-    buf = _op_scratch(device or torch.cuda.current_device())
-    try:
-        _lib.check(_lib.load().qb_op_check(buf.data_ptr(), _lib.stream_handle()))
-    except Exception:
-        _workspaces.clear()  # a kernel that gave up may have left its tickets mid-count
-        raise
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    with torch.cuda.device(device):
+        buf = _op_scratch(torch.device("cuda", torch.cuda.current_device()))
+        try:
+            _lib.check(_lib.load().qb_op_check(buf.data_ptr(), _lib.stream_handle()))
+        except Exception:
+            _workspaces.clear()  # a kernel that gave up may have left its tickets mid-count
+            raise
 
 
 def norm_projection(x, gain, weight, eps=1e-6, *, swiglu=False):
@@ -181,6 +183,12 @@ def rope_attention(qkv, q_norm, k_norm, cos, sin, keys, values, position, eps=1e
 # workspace, and a call made while a graph is captured takes one from the
 # graph's own memory, so graphs share none either.
 
+I32 = torch.int32
+_raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
+    lambda index: torch.cuda.current_stream(index).cuda_stream)
+_workspace_bytes = {}
+
+
 def _status(device) -> int:
     """Address of the device error word that ``check_device_errors`` reads."""
     buf = _scratch.get(device.index)
@@ -191,47 +199,59 @@ def _status(device) -> int:
     return buf.data_ptr()
 
 
-def _workspace(device, stream: int, nbytes: int) -> torch.Tensor:
-    zero = 8192  # qb_paged_zero_bytes()
+def _workspace(device, stream: int, max_queries: int, hq: int, hkv: int, prefix_tokens: int):
+    """Workspace of a paged call: (the tensor, its size in bytes)."""
+    key = (device.index, max_queries, hq, hkv, prefix_tokens)
+    nbytes = _workspace_bytes.get(key)
+    if nbytes is None:
+        n = _lib.c_size_t()
+        _lib.check(_lib.load().qb_paged_workspace_bytes(max_queries, hq, hkv, prefix_tokens, _lib.ctypes.byref(n)))
+        if len(_workspace_bytes) > 4096:
+            _workspace_bytes.clear()
+        nbytes = _workspace_bytes[key] = n.value
     if torch.cuda.is_current_stream_capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        buf[:zero].zero_()
-        return buf
-    key = (device.index, stream)
-    buf = _workspaces.get(key)
+        buf[:8192].zero_()  # qb_paged_zero_bytes()
+        return buf, nbytes
+    buf = _workspaces.get((device.index, stream))
     if buf is None or buf.numel() < nbytes:
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        buf[:zero].zero_()
-        _workspaces[key] = buf
-    return buf
+        buf[:8192].zero_()
+        _workspaces[device.index, stream] = buf
+    return buf, nbytes
 
 
 def _on(device):
     """Make ``device`` current for the call (the library launches there)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+    return _SAME if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+
+
+_SAME = contextlib.nullcontext()
 
 
 def _batch(device, k_pages, v_pages, page_table, q_start, kv_lens):
     """Checked (pages, Hkv, page, table width, sequences) of a paged batch."""
-    _require(k_pages.dim() == 4 and k_pages.shape == v_pages.shape and k_pages.shape[3] == 128,
-             "expected k_pages and v_pages [pages, Hkv, page, 128]")
-    for t in (k_pages, v_pages):
-        _require(t.dtype == BF16 and t.device == device and t.is_contiguous(),
-                 "expected contiguous bf16 pools on the device of the queries")
-    for t in (page_table, q_start, kv_lens):
-        _require(t.dtype == torch.int32 and t.device == device and t.is_contiguous(),
-                 "page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the queries")
-    _require(page_table.dim() == 2 and kv_lens.dim() == 1 and q_start.dim() == 1
-             and page_table.shape[0] == kv_lens.shape[0] and q_start.shape[0] == kv_lens.shape[0] + 1,
-             "expected page_table [B, P], q_start [B + 1], kv_lens [B]")
-    return (*k_pages.shape[:3], page_table.shape[1], kv_lens.shape[0])
+    shape = k_pages.shape
+    if len(shape) != 4 or shape[3] != 128 or v_pages.shape != shape:
+        raise ValueError("expected k_pages and v_pages [pages, Hkv, page, 128]")
+    if not (k_pages.dtype == BF16 and v_pages.dtype == BF16 and k_pages.is_contiguous() and v_pages.is_contiguous()
+            and k_pages.device == device and v_pages.device == device):
+        raise ValueError("expected contiguous bf16 pools on the device of the queries")
+    if not (page_table.dtype == I32 and q_start.dtype == I32 and kv_lens.dtype == I32 and page_table.is_contiguous()
+            and q_start.is_contiguous() and kv_lens.is_contiguous() and page_table.device == device
+            and q_start.device == device and kv_lens.device == device):
+        raise ValueError("page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the queries")
+    table, seqs = page_table.shape, kv_lens.shape
+    if len(table) != 2 or len(seqs) != 1 or table[0] != seqs[0] or q_start.shape != (seqs[0] + 1,):
+        raise ValueError("expected page_table [B, P], q_start [B + 1], kv_lens [B]")
+    return shape[0], shape[1], shape[2], table[1], seqs[0]
 
 
 def _rows_out(out, shape, device):
     if out is None:
         return torch.empty(shape, dtype=BF16, device=device)
-    _require(out.dtype == BF16 and out.device == device and out.is_contiguous() and tuple(out.shape) == tuple(shape),
-             "out must be a contiguous bf16 tensor of the result's shape on the device of the queries")
+    if not (out.dtype == BF16 and out.device == device and out.is_contiguous() and out.shape == shape):
+        raise ValueError("out must be a contiguous bf16 tensor of the result's shape on the device of the queries")
     return out
 
 
@@ -267,7 +287,7 @@ def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_tabl
             qkv.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), cos.data_ptr(), sin.data_ptr(), cos.shape[0], float(eps),
             k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width, q_start.data_ptr(),
             kv_lens.data_ptr(), seqs, tokens, int(first_position), hq, hkv, out.data_ptr(), _status(dev),
-            _lib.stream_handle()))
+            _raw_stream(dev.index)))
     return out
 
 
@@ -294,9 +314,8 @@ def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0,
         max_queries = tokens
     with _on(dev):
         out = _rows_out(out, q.shape, dev)
-        need = _paged_bytes(max_queries, hq, hkv, 0)
-        stream = _lib.stream_handle()
-        ws = _workspace(dev, stream, need)
+        stream = _raw_stream(dev.index)
+        ws, need = _workspace(dev, stream, max_queries, hq, hkv, 0)
         _lib.check(_lib.load().qb_paged_attention(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
             q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, int(max_queries), hq, hkv, int(window), int(sinks),
@@ -323,21 +342,14 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
         max_queries = tokens
     with _on(dev):
         out = _rows_out(out, q.shape, dev)
-        need = _paged_bytes(max_queries, hq, hkv, tokens)
-        stream = _lib.stream_handle()
-        ws = _workspace(dev, stream, need)
+        stream = _raw_stream(dev.index)
+        ws, need = _workspace(dev, stream, max_queries, hq, hkv, tokens)
         _lib.check(_lib.load().qb_shared_prefix_attention(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, prefix_table.data_ptr(),
             prefix_table.shape[0], int(prefix_len), page_table.data_ptr(), width, q_start.data_ptr(),
             kv_lens.data_ptr(), seqs, tokens, int(max_queries), hq, hkv, out.data_ptr(), ws.data_ptr(), need,
             _status(dev), stream))
     return out
-
-
-def _paged_bytes(max_queries, hq, hkv, prefix_tokens) -> int:
-    n = _lib.c_size_t()
-    _lib.check(_lib.load().qb_paged_workspace_bytes(max_queries, hq, hkv, prefix_tokens, _lib.ctypes.byref(n)))
-    return n.value
 
 
 def _setting(value, name, rows, dtype, device, lo, hi):
@@ -381,5 +393,5 @@ def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
                  "out must be a contiguous int64 tensor [R] on the device of the logits")
         _lib.check(_lib.load().qb_sample_token(logits.data_ptr(), int(logits.dtype == torch.float32), rows, vocab,
                                                uniforms.data_ptr(), t, t_all, k, k_all, p, p_all, m, m_all,
-                                               out.data_ptr(), _status(dev), _lib.stream_handle()))
+                                               out.data_ptr(), _status(dev), _raw_stream(dev.index)))
     return out
