@@ -88,10 +88,13 @@ struct AppendArgs {
 };
 
 constexpr int kAppThreads = 256;
+constexpr int kAppHeads = 4;  // heads that a half-warp holds at once: 64 of a token
 
 // One CTA per token: 16 half-warps take the token's Hq + 2 Hkv heads in turn,
-// lane j of a half-warp the dims [8j, 8j + 8) of its head (one 16-byte access
-// each way; the rotation's partner dim d +- 64 is lane j ^ 8).
+// lane j of a half-warp the dims [8j, 8j + 8) of its heads (one 16-byte access
+// each way; the rotation's partner dim d +- 64 is lane j ^ 8). Bound by bytes:
+// the token's heads are on their way before its sequence, position and page are
+// looked up (three dependent reads).
 //   y = x * (1 / sqrt(mean(x^2) + eps)) * gain,  out = y * cos + rot_half(y) * sin
 // in fp32 with one rounding at the end (rope_attention rounds every product,
 // as the reference does; the cache rows of the two may differ by an ulp).
@@ -101,7 +104,16 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
   const int t = blockIdx.x;
   const int hw = threadIdx.x >> 4, j = threadIdx.x & 15;
   const int heads = a.Hq + 2 * a.Hkv;
-  const bf16* row = a.qkv + (size_t)t * heads * kAttnD;
+  const bf16* row = a.qkv + (size_t)t * heads * kAttnD + 8 * j;
+  uint4 xv[kAppHeads];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int i = 0; i < kAppHeads; ++i) {
+      const int h = h0 + 16 * i + hw;
+      xv[i] = h < heads ? ld128(row + (size_t)h * kAttnD) : make_uint4(0, 0, 0, 0);
+    }
+  };
+  load(0);
   // the sequence that holds token t: the count of starts (from the second) at or below t
   int seq = 0;
   for (int s0 = 0; s0 < a.b.n_seqs; s0 += kAppThreads) {
@@ -117,55 +129,61 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
     if (threadIdx.x == 0) report_error(a.err, DEV_BAD_POSITION);
     return;
   }
+  const uint4 cv = ld128(a.cos + (size_t)angle * kAttnD + 8 * j);
+  const uint4 sv = ld128(a.sin + (size_t)angle * kAttnD + 8 * j);
   const int page = a.b.page_table[(size_t)seq * a.b.table_width + (pos >> a.b.page_log2)];
   const bool page_ok = page >= 0 && page < a.b.num_pages;
   if (!page_ok && threadIdx.x == 0) report_error(a.err, DEV_BAD_PAGE);
   const int slot = pos & ((1 << a.b.page_log2) - 1);
-  const uint4 cv = ld128(a.cos + (size_t)angle * kAttnD + 8 * j);
-  const uint4 sv = ld128(a.sin + (size_t)angle * kAttnD + 8 * j);
   const uint32_t c2[4] = {cv.x, cv.y, cv.z, cv.w}, s2[4] = {sv.x, sv.y, sv.z, sv.w};
-  for (int h0 = 0; h0 < heads; h0 += kAppThreads / 16) {
-    const int h = h0 + hw;
-    const bool live = h < heads;
-    uint4 xv = live ? ld128(row + (size_t)h * kAttnD + 8 * j) : make_uint4(0, 0, 0, 0);
-    const bool turn = live && h < a.Hq + a.Hkv;
-    const bf16* gain = h < a.Hq ? a.q_norm : a.k_norm;
-    float x[8] = {bf_lo(xv.x), bf_hi(xv.x), bf_lo(xv.y), bf_hi(xv.y), bf_lo(xv.z), bf_hi(xv.z), bf_lo(xv.w), bf_hi(xv.w)};
-    float ss = 0.f;
+  for (int h0 = 0; h0 < heads; h0 += 16 * kAppHeads) {
+    if (h0 > 0) load(h0);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+    for (int i = 0; i < kAppHeads; ++i) {
+      const int h = h0 + 16 * i + hw;
+      if (h0 + 16 * i >= heads) break;
+      const bool turn = h < a.Hq + a.Hkv;
+      const bf16* gain = h < a.Hq ? a.q_norm : a.k_norm;
+      float x[8] = {bf_lo(xv[i].x), bf_hi(xv[i].x), bf_lo(xv[i].y), bf_hi(xv[i].y),
+                    bf_lo(xv[i].z), bf_hi(xv[i].z), bf_lo(xv[i].w), bf_hi(xv[i].w)};
+      float ss = 0.f;
 #pragma unroll
-    for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-    if (turn && gain != nullptr) {
-      const float inv = 1.0f / sqrtf(ss / (float)kAttnD + a.eps);
-      const uint4 gv = ld128(gain + 8 * j);
-      const uint32_t g2[4] = {gv.x, gv.y, gv.z, gv.w};
+      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x[2 * i] = x[2 * i] * inv * bf_lo(g2[i]);
-        x[2 * i + 1] = x[2 * i + 1] * inv * bf_hi(g2[i]);
+      for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      if (turn && gain != nullptr) {
+        const float inv = 1.0f / sqrtf(ss / (float)kAttnD + a.eps);
+        const uint4 gv = ld128(gain + 8 * j);
+        const uint32_t g2[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          x[2 * e] = x[2 * e] * inv * bf_lo(g2[e]);
+          x[2 * e + 1] = x[2 * e + 1] * inv * bf_hi(g2[e]);
+        }
       }
-    }
-    float o[8];
+      float o[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float other = __shfl_xor_sync(0xffffffffu, x[i], 8);
-      const float c = (i & 1) ? bf_hi(c2[i >> 1]) : bf_lo(c2[i >> 1]);
-      const float s = (i & 1) ? bf_hi(s2[i >> 1]) : bf_lo(s2[i >> 1]);
-      o[i] = turn ? fmaf(x[i], c, (j < 8 ? -other : other) * s) : x[i];
+      for (int e = 0; e < 8; ++e) {
+        const float other = __shfl_xor_sync(0xffffffffu, x[e], 8);
+        const float c = (e & 1) ? bf_hi(c2[e >> 1]) : bf_lo(c2[e >> 1]);
+        const float s = (e & 1) ? bf_hi(s2[e >> 1]) : bf_lo(s2[e >> 1]);
+        o[e] = fmaf(x[e], c, (j < 8 ? -other : other) * s);
+      }
+      if (h >= heads) continue;
+      const uint4 ov = turn ? make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]),
+                                         pack_bf16(o[6], o[7]))
+                            : xv[i];
+      bf16* dst;
+      if (h < a.Hq) {
+        dst = a.q_out + ((size_t)t * a.Hq + h) * kAttnD;
+      } else {
+        if (!page_ok) continue;
+        const int kh = turn ? h - a.Hq : h - a.Hq - a.Hkv;
+        bf16* pool = turn ? a.k_pages : a.v_pages;
+        dst = pool + ((((size_t)page * a.Hkv + kh) << a.b.page_log2) + slot) * kAttnD;
+      }
+      *reinterpret_cast<uint4*>(dst + 8 * j) = ov;
     }
-    if (!live) continue;
-    const uint4 ov = turn ? make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7])) : xv;
-    bf16* dst;
-    if (h < a.Hq) {
-      dst = a.q_out + ((size_t)t * a.Hq + h) * kAttnD;
-    } else {
-      if (!page_ok) continue;
-      const int kh = h - a.Hq < a.Hkv ? h - a.Hq : h - a.Hq - a.Hkv;
-      bf16* pool = h - a.Hq < a.Hkv ? a.k_pages : a.v_pages;
-      dst = pool + ((((size_t)page * a.Hkv + kh) << a.b.page_log2) + slot) * kAttnD;
-    }
-    *reinterpret_cast<uint4*>(dst + 8 * j) = ov;
   }
 }
 

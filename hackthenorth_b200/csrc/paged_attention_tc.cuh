@@ -41,9 +41,12 @@ constexpr int kPtTile = 128 * 128 * 2;         // a Q tile: 32 KB, dims 0-63 the
 constexpr int kPtKvTile = kPtKeys * 128 * 2;   // a K or V tile: 16 KB, likewise
 constexpr int kPtSlots = 4;                    // ring slots of each
 constexpr int kPtMaxUnits = 4096;
+constexpr int kPagedMaxTcCtas = 1024;
 constexpr int kPtMinTiles = 2;
+constexpr int kPtUnitCost = 4;  // what beginning and ending a unit takes, in key tiles: its place in the line
 
 constexpr int kPtPieces = 4;
+constexpr int kPtPolyEvery = 3;  // every third pair of P comes from exp2_poly, the rest from the MUFU
 
 // What a CTA does next: the key tiles [k0, k1) of a unit (a role's whole state).
 struct PtPiece {
@@ -183,6 +186,30 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer, a
+// cubic for 2^f on [-1/2, 1/2] (fitted to the least largest relative error,
+// 2^-13.7, beside P's rounding of 2^-9), n added to the exponent. x is held at
+// -125 or more, so that the result stays a normal number; a NaN becomes the
+// largest finite one.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& p0, float& p1) {
+  constexpr float kC0 = 0.99992807f, kC1 = 0.69326099f, kC2 = 0.24261113f, kC3 = 0.05517167f;
+  float a, b;
+  unpack_f32x2(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-125.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-125.f));
+  x = f32x2(a, b);
+  const uint64_t n = add_f32x2(x, f32x2(12582912.f, 12582912.f));  // 1.5 * 2^23: the sum's low bits are n
+  const uint64_t f = add_f32x2(x, fma_f32x2(n, f32x2(-1.f, -1.f), f32x2(12582912.f, 12582912.f)));
+  uint64_t p = fma_f32x2(f, f32x2(kC3, kC3), f32x2(kC2, kC2));
+  p = fma_f32x2(p, f, f32x2(kC1, kC1));
+  p = fma_f32x2(p, f, f32x2(kC0, kC0));
+  float n0, n1;
+  unpack_f32x2(n, n0, n1);
+  unpack_f32x2(p, p0, p1);
+  p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
+  p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+}
+
 // A word with its lowest n bits set (n clamped to 0..32).
 __device__ __forceinline__ uint32_t bits_below(int n) { return n <= 0 ? 0u : n >= 32 ? 0xffffffffu : (1u << n) - 1u; }
 
@@ -262,7 +289,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   PtPiece* pieces = reinterpret_cast<PtPiece*>(bars + 64);
   SeqSpan* seqs = reinterpret_cast<SeqSpan*>(pieces + kPtPieces);
   int* seq_unit = reinterpret_cast<int*>(seqs + kPagedMaxSeqs);  // [n_seqs + 1] units before each sequence
-  int* unit_tile = seq_unit + kPagedMaxSeqs + 1;          // [units + 1] tiles before each unit
+  int* unit_tile = seq_unit + kPagedMaxSeqs + 1;          // [units + 1] the line before each unit (of one head)
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
   const int RH = 128 / a.G;  // tokens per M tile
@@ -326,12 +353,12 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   int tiles = 0;
   for (int u0 = 0; u0 < units; u0 += kPtThreads) {
     const int u = u0 + threadIdx.x;
-    const int v = block_scan(u < units ? tc_unit(b, seqs, seq_unit, u, 2 * RH).ts.count : 0, warp_tot, tiles);
+    const int v = block_scan(u < units ? tc_unit(b, seqs, seq_unit, u, 2 * RH).ts.count + kPtUnitCost : 0, warp_tot, tiles);
     if (u < units) unit_tile[u + 1] = v;
   }
   __syncthreads();
   const long long total = (long long)tiles * a.Hkv;
-  const int E = (int)min((long long)gridDim.x, max(1ll, total / kPtMinTiles));
+  const int E = (int)min((long long)gridDim.x, max(1ll, (total - (long long)units * a.Hkv * kPtUnitCost) / kPtMinTiles));
   const int me = blockIdx.x;
   const bool busy = me < E && total > 0;
   const long long t_begin = busy ? tile_begin(me, total, E) : 0, t_end = busy ? tile_begin(me + 1, total, E) : 0;
@@ -436,7 +463,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         const int e = made % kPtPieces;
         PtPiece p;
         p.k0 = p.k1 = 0;  // the end of the CTA's work
-        if (at < t_end) {
+        while (at < t_end && p.k0 == p.k1) {
           if (fresh != u) {
             un = tc_unit(b, seqs, seq_unit, u, 2 * RH);
             n = unit_tile[u + 1] - unit_tile[u];
@@ -454,13 +481,14 @@ __global__ void __launch_bounds__(kPtThreads, 1)
           p.n_sink = un.ts.n_sink;
           p.lo = un.ts.lo;
           p.head = g;
-          p.k0 = (int)(at - u0);
-          p.k1 = (int)min((long long)n, p.k0 + (t_end - at));
-          p.whole = p.k0 == 0 && p.k1 == n;
+          const int x0 = (int)(at - u0), x1 = (int)min((long long)n, x0 + (t_end - at));
+          p.k0 = max(0, x0 - kPtUnitCost);  // its first places hold no tile
+          p.k1 = max(0, x1 - kPtUnitCost);
+          p.whole = p.k0 == 0 && x1 == n;
           p.first = at == t_begin;
           p.last = p.k0 == 0 && !p.whole ? tile_owner(u0 + n - 1, total, E) : -1;
-          at += p.k1 - p.k0;
-          if (g == a.Hkv - 1 && p.k1 == n) ++u;
+          at += x1 - x0;
+          if (g == a.Hkv - 1 && x1 == n) ++u;
         }
         if (made >= kPtPieces)
           ok = __all_sync(0xffffffffu, mbar_wait(&piece_empty[e], ((made / kPtPieces) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY));
@@ -596,7 +624,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       for (int k = k0; k < k1; ++k, ++J) {
         const int c0 = tile_key(un, k);
         const uint32_t buf = s_col + 64 * (J & 1);
-        bool ok = mbar_wait(&s_full[2 * t + (J & 1)], (sphase >> (J & 1)) & 1, a.err, DEV_TIMEOUT_ATTN_FULL) && flags[0] == 0;
+        bool ok = pt_wait(&s_full[2 * t + (J & 1)], (sphase >> (J & 1)) & 1, a.err, DEV_TIMEOUT_ATTN_FULL);
         if (!__all_sync(0xffffffffu, ok)) return false;
         sphase ^= 1u << (J & 1);
         tc_fence_after();
@@ -673,9 +701,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         for (int c = 0; c < 64; c += 2) {
           const uint64_t x = fma_f32x2(f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, mu2);
           float p0, p1;
-          unpack_f32x2(x, p0, p1);
-          p0 = ex2_approx(p0);
-          p1 = ex2_approx(p1);
+          if ((c >> 1) % kPtPolyEvery == kPtPolyEvery - 1) {
+            exp2_poly(x, p0, p1);
+          } else {
+            unpack_f32x2(x, p0, p1);
+            p0 = ex2_approx(p0);
+            p1 = ex2_approx(p1);
+          }
           rs[(c >> 1) & 1] = add_f32x2(rs[(c >> 1) & 1], f32x2(p0, p1));
           sr[c >> 1] = pack_bf16(p0, p1);
         }
@@ -692,6 +724,7 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const bool ok = pv_done(J - 1);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
+      if (m_ref == -INFINITY) l = 0.f;  // nothing seen: exp2_poly leaves 2^-125 where the mask is -inf
       const bool whole = un.whole != 0;
       const int slot = 2 * me + (un.first ? 0 : 1);
       const size_t row = (size_t)(un.token0 + token) * a.Hq + un.head * a.G + hj;
@@ -767,21 +800,39 @@ __global__ void __launch_bounds__(kPtThreads, 1)
   }
 }
 
-// Joins the pieces of the units that paged_tc_kernel cut: blockIdx.x is the
-// CTA whose last piece begins the unit, blockIdx.y takes 32 of its rows, a
-// warp a row at a time, a lane 4 dims. Bytes: the pieces once (L2).
-constexpr int kPjRows = 32;
+// Joins the pieces of the units that paged_tc_kernel cut: a warp a row, a lane
+// 4 dims, the rows of all cut units dealt out to the grid's warps. Bound by the
+// latency of its loads (the pieces lie in L2), so a row's are issued eight
+// pieces at a time.
 constexpr int kPjThreads = 256;
-__global__ void __launch_bounds__(kPjThreads) paged_join_kernel(const PagedTcArgs a) {
+constexpr int kPjCtasPerSm = 8;
+__global__ void __launch_bounds__(kPjThreads) paged_join_kernel(const PagedTcArgs a, int ctas) {
+  __shared__ int cut_of[kPagedMaxTcCtas];
+  __shared__ int warp_cuts[kPjThreads / 32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  const PtUnit un = a.cut[blockIdx.x];
-  if (!un.valid) return;
-  const int RH = 128 / a.G, first = blockIdx.x;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  int cuts = 0;
+  for (int c0 = 0; c0 < ctas; c0 += kPjThreads) {  // the CTAs whose last piece begins a cut unit
+    const int c = c0 + threadIdx.x;
+    const bool is = c < ctas && a.cut[c].valid != 0;
+    const unsigned who = __ballot_sync(0xffffffffu, is);
+    if (lane == 0) warp_cuts[warp] = __popc(who);
+    __syncthreads();
+    int at = cuts;
+    for (int w = 0; w < kPjThreads / 32; ++w) {
+      if (w < warp) at += warp_cuts[w];
+      cuts += warp_cuts[w];
+    }
+    if (is) cut_of[at + __popc(who & ((1u << lane) - 1u))] = c;
+    __syncthreads();
+  }
+  const int RH = 128 / a.G;
   const bool has_base = a.sink.base32 != nullptr;
-  for (int i = warp; i < kPjRows; i += kPjThreads / 32) {
-    const int r = blockIdx.y * kPjRows + i, t = r >> 7, qrow = r & 127;
+  for (int i = blockIdx.x * (kPjThreads / 32) + warp; i < cuts * kPtRows; i += gridDim.x * (kPjThreads / 32)) {
+    const int first = cut_of[i / kPtRows];
+    const PtUnit un = a.cut[first];
+    const int r = i % kPtRows, t = r >> 7, qrow = r & 127;
     const int qi = qrow / a.G, token = t * RH + qi;
     if (qi >= RH || token >= un.tokens) continue;
     auto piece = [&](int c) { return (size_t)(2 * c + (c == first ? un.first_slot : 0)) * kPtRows + r; };
@@ -791,16 +842,25 @@ __global__ void __launch_bounds__(kPjThreads) paged_join_kernel(const PagedTcArg
     const float mu = top == -INFINITY ? 0.f : top;
     float lsum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = first; c <= un.last; ++c) {
-      const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + piece(c) * 2);
-      const float4 ov = *reinterpret_cast<const float4*>(a.part_o + piece(c) * kAttnD + 4 * lane);
-      const float w = exp2f(ml.x - mu);
-      lsum = fmaf(ml.y, w, lsum);
-      acc.x = fmaf(ov.x, w, acc.x);
-      acc.y = fmaf(ov.y, w, acc.y);
-      acc.z = fmaf(ov.z, w, acc.z);
-      acc.w = fmaf(ov.w, w, acc.w);
+    for (int c0 = first; c0 <= un.last; c0 += 8) {
+      float2 ml[8];
+      float4 ov[8];
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const bool in = c0 + j <= un.last;
+        ml[j] = in ? *reinterpret_cast<const float2*>(a.part_ml + piece(c0 + j) * 2) : make_float2(-INFINITY, 0.f);
+        ov[j] = in ? *reinterpret_cast<const float4*>(a.part_o + piece(c0 + j) * kAttnD + 4 * lane)
+                   : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        const float w = exp2f(ml[j].x - mu);
+        lsum = fmaf(ml[j].y, w, lsum);
+        acc.x = fmaf(ov[j].x, w, acc.x);
+        acc.y = fmaf(ov[j].y, w, acc.y);
+        acc.z = fmaf(ov[j].z, w, acc.z);
+        acc.w = fmaf(ov[j].w, w, acc.w);
+      }
     }
     const size_t row = (size_t)(un.token0 + token) * a.Hq + un.head * a.G + qrow % a.G;
     const RowScale rs = row_scale(top, lsum, has_base, has_base ? a.sink.base_lse[row] : 0.f);

@@ -104,7 +104,7 @@ __device__ __forceinline__ long long tile_begin(int i, long long total, int E) {
 
 __host__ inline size_t pd_smem_bytes() {
   return 1024 + (size_t)kPdStages * kPdStageBytes + kPdRows * kPdPStride + 2 * kPdWarps * kPdRows * 4 +
-         2 * kPdStages * 8 + 64 + (kPagedMaxSeqs + 1) * 4;
+         2 * kPdStages * 8 + 64 + (kPagedMaxSeqs + 1) * 4 + 4 + kPagedMaxSeqs * 8;
 }
 
 __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
@@ -120,6 +120,8 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
   int* flag = reinterpret_cast<int*>(empty + kPdStages);                 // [0]: this CTA joins the unit's pieces
   int* warp_tot = flag + 1;                                              // [5]
   int* pref = flag + 16;                                                 // [n_seqs + 1] tiles before each sequence
+  // First row and queries (at most 16) in one word, and keys, of each sequence: a new one costs no trip to memory.
+  int2* seqs = reinterpret_cast<int2*>(pref + kPagedMaxSeqs + 2);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const PagedBatch& b = a.b;
 
@@ -142,6 +144,7 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
     int cnt = 0;
     if (s < b.n_seqs) {
       const SeqSpan sp = paged_seq(b, s, a.err);
+      seqs[s] = make_int2(sp.q0 | sp.n << 25, sp.kv);
       if (sp.n > 0) cnt = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks).count;
     }
     int v = cnt;
@@ -192,7 +195,7 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
     for (long long t = t_begin; t < t_end && ok; ++seq) {
       const int n_tiles = pref[seq + 1] - pref[seq];
       if (n_tiles == 0) continue;
-      const SeqSpan sp = paged_seq(b, seq, nullptr);
+      const SeqSpan sp = {seqs[seq].x & 0x1ffffff, seqs[seq].x >> 25, seqs[seq].y};
       const TileSpan ts = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks);
       const long long base = (long long)pref[seq] * a.Hkv;
       const long long stop = min(t_end, base + (long long)n_tiles * a.Hkv);
@@ -243,7 +246,7 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
   for (long long t = t_begin; t < t_end; ++seq) {
     const int n_tiles = pref[seq + 1] - pref[seq];
     if (n_tiles == 0) continue;
-    const SeqSpan sp = paged_seq(b, seq, nullptr);
+    const SeqSpan sp = {seqs[seq].x & 0x1ffffff, seqs[seq].x >> 25, seqs[seq].y};
     const TileSpan ts = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks);
     const long long base = (long long)pref[seq] * a.Hkv;
     const long long stop = min(t_end, base + (long long)n_tiles * a.Hkv);

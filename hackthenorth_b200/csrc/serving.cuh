@@ -54,7 +54,7 @@ PagedWorkspace paged_workspace(int grid, int rows, long long base_rows) {
   return w;
 }
 int decode_grid() { return std::min(current_sm_count() * kPdCtasPerSm, kPagedMaxCtas); }
-int tc_grid() { return std::min(current_sm_count(), kPagedMaxCtas); }
+int tc_grid() { return std::min(current_sm_count(), kPagedMaxTcCtas); }
 
 // Whether the few-rows kernel takes the call: its 16 MMA rows hold every
 // sequence's query rows of a KV head.
@@ -104,7 +104,7 @@ cudaError_t launch_paged_tc(const CUtensorMap& q, const CUtensorMap& k, const CU
   const int grid = tc_grid();
   e = launch_ex(paged_tc_kernel, dim3(grid), dim3(kPtThreads), pt_smem_bytes(a.max_units), st, q, k, v, a);
   if (e != cudaSuccess) return e;
-  return launch_ex(paged_join_kernel, dim3(grid, kPtRows / kPjRows), dim3(kPjThreads), 0, st, a);
+  return launch_ex(paged_join_kernel, dim3(grid * kPjCtasPerSm), dim3(kPjThreads), 0, st, a, grid);
 }
 
 int check_tiles(int tokens, int n_seqs, int G, int table_width, int page_size) {
