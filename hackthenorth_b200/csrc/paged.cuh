@@ -95,7 +95,7 @@ constexpr int kAppHeads = 4;  // heads that a half-warp holds at once: 64 of a t
 // each way; the rotation's partner dim d +- 64 is lane j ^ 8). Bound by bytes:
 // the token's heads are on their way before its sequence, position and page are
 // looked up (three dependent reads).
-//   y = x * (1 / sqrt(mean(x^2) + eps)) * gain,  out = y * cos + rot_half(y) * sin
+//   y = x * rsqrt(mean(x^2) + eps) * gain,  out = y * cos + rot_half(y) * sin
 // in fp32 with one rounding at the end (rope_attention rounds every product,
 // as the reference does; the cache rows of the two may differ by an ulp).
 __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendArgs a) {
@@ -130,7 +130,9 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
     return;
   }
   const uint4 cv = ld128(a.cos + (size_t)angle * kAttnD + 8 * j);
-  const uint4 sv = ld128(a.sin + (size_t)angle * kAttnD + 8 * j);
+  uint4 sv = ld128(a.sin + (size_t)angle * kAttnD + 8 * j);
+  const uint32_t sign = j < 8 ? 0x80008000u : 0u;  // the first half takes minus the second
+  sv.x ^= sign; sv.y ^= sign; sv.z ^= sign; sv.w ^= sign;
   const int page = a.b.page_table[(size_t)seq * a.b.table_width + (pos >> a.b.page_log2)];
   const bool page_ok = page >= 0 && page < a.b.num_pages;
   if (!page_ok && threadIdx.x == 0) report_error(a.err, DEV_BAD_PAGE);
@@ -146,28 +148,30 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
       const bf16* gain = h < a.Hq ? a.q_norm : a.k_norm;
       float x[8] = {bf_lo(xv[i].x), bf_hi(xv[i].x), bf_lo(xv[i].y), bf_hi(xv[i].y),
                     bf_lo(xv[i].z), bf_hi(xv[i].z), bf_lo(xv[i].w), bf_hi(xv[i].w)};
-      float ss = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
-#pragma unroll
-      for (int o = 8; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-      if (turn && gain != nullptr) {
-        const float inv = 1.0f / sqrtf(ss / (float)kAttnD + a.eps);
-        const uint4 gv = ld128(gain + 8 * j);
-        const uint32_t g2[4] = {gv.x, gv.y, gv.z, gv.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          x[2 * e] = x[2 * e] * inv * bf_lo(g2[e]);
-          x[2 * e + 1] = x[2 * e + 1] * inv * bf_hi(g2[e]);
-        }
-      }
       float o[8];
+      if (__any_sync(0xffffffffu, turn)) {  // a warp of V heads only copies
+        float ss = 0.f;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float other = __shfl_xor_sync(0xffffffffu, x[e], 8);
-        const float c = (e & 1) ? bf_hi(c2[e >> 1]) : bf_lo(c2[e >> 1]);
-        const float s = (e & 1) ? bf_hi(s2[e >> 1]) : bf_lo(s2[e >> 1]);
-        o[e] = fmaf(x[e], c, (j < 8 ? -other : other) * s);
+        for (int e = 0; e < 8; ++e) ss = fmaf(x[e], x[e], ss);
+#pragma unroll
+        for (int d = 8; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
+        if (turn && gain != nullptr) {
+          const float inv = rsqrtf(ss * (1.0f / kAttnD) + a.eps);  // within 2^-22; the one rounding at the end is 2^-9
+          const uint4 gv = ld128(gain + 8 * j);
+          const uint32_t g2[4] = {gv.x, gv.y, gv.z, gv.w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x[2 * e] = x[2 * e] * inv * bf_lo(g2[e]);
+            x[2 * e + 1] = x[2 * e + 1] * inv * bf_hi(g2[e]);
+          }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float other = __shfl_xor_sync(0xffffffffu, x[e], 8);
+          const float c = (e & 1) ? bf_hi(c2[e >> 1]) : bf_lo(c2[e >> 1]);
+          const float s = (e & 1) ? bf_hi(s2[e >> 1]) : bf_lo(s2[e >> 1]);
+          o[e] = fmaf(x[e], c, other * s);  // s carries the sign
+        }
       }
       if (h >= heads) continue;
       const uint4 ov = turn ? make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]),
