@@ -24,6 +24,7 @@ import torch
 
 from . import _lib
 from .config import ModelConfig
+from .sampling import Sampling
 from .weights import PackedWeights, load_checkpoint, random_state_dict, rotary_table
 
 BF16 = torch.bfloat16
@@ -95,20 +96,24 @@ class DecodeState:
     Capacity = prompt_length + output_length - 1 + draft slots. The caches are
     zero-filled (finite), laid out ``[L, Hkv, capacity, D]``; with ``batch`` B > 1
     sequences (one GPU, B <= 8) ``[L, B, Hkv, capacity, D]``, and ``token`` /
-    ``position`` hold one entry per sequence.
+    ``position`` hold one entry per sequence. With ``sampling``, ``prefill`` and
+    ``step`` draw ``token`` from the logits (``ops.sample_token``) in place of the
+    greedy one.
     """
 
     MAX_BATCH = 8
 
     def __init__(self, engine: "Engine", prompt_length: int, output_length: int,
                  draft_tokens: int = 0, keep_logits: bool = False, capacity: Optional[int] = None,
-                 batch: int = 1):
+                 batch: int = 1, sampling: Optional[Sampling] = None):
         cfg = engine.cfg
         dev = engine.device
         if not 1 <= batch <= self.MAX_BATCH:
             raise ValueError(f"batch must lie in 1..{self.MAX_BATCH}")
         if batch > 1 and engine.tp_size > 1:
             raise ValueError("batched decode runs on one GPU")
+        if sampling is not None and engine.tp_size > 1:
+            raise ValueError("sampling runs on one GPU")
         self.engine = engine
         self.batch = batch
         self.draft_tokens = draft_tokens
@@ -130,13 +135,37 @@ class DecodeState:
         self.prompt = torch.zeros(batch * max(prompt_length, 1), dtype=torch.int64, device=dev)
         # this rank's vocabulary shard under tensor parallelism; [B, V] batched
         vshape = (cfg.vocab // engine.tp_size,) if batch == 1 else (batch, cfg.vocab)
-        self.logits = torch.zeros(vshape, dtype=BF16, device=dev) if keep_logits else None
+        self.logits = torch.zeros(vshape, dtype=BF16, device=dev) if keep_logits or sampling is not None else None
+        self.set_sampling(sampling)
         _lib.check(L.qb_set_batch(engine.ctx, batch), engine.ctx)
         _lib.check(L.qb_bind_state(engine.ctx, self.keys.data_ptr(), self.values.data_ptr(), self.capacity,
                                    self.cos.data_ptr(), self.sin.data_ptr(), self.workspace.data_ptr(),
                                    self.workspace.numel()), engine.ctx)
         engine._bound_state = self
         self.captured = False
+
+    def set_sampling(self, sampling: Optional[Sampling], lane: int = 0) -> None:
+        """Settings of the tokens drawn from here on, from the beginning of their
+        seed's numbers (``lane``: which of several states shares the seed). A
+        state made without ``sampling`` takes none."""
+        if sampling is not None and self.logits is None:
+            raise ValueError("this DecodeState was made without sampling")
+        self.sampling = sampling
+        if sampling is not None:
+            dev = self.token.device
+            self._numbers = torch.Generator(device=dev)
+            self._numbers.manual_seed((sampling.seed + lane * 0x9E3779B1) % 2 ** 63)
+            self._uniforms = torch.empty(self.batch, dtype=torch.float32, device=dev)
+
+    def _draw(self) -> None:
+        """Replace the greedy ``token`` by a drawn one."""
+        if self.sampling is None:
+            return
+        from . import ops
+
+        s = self.sampling
+        self._uniforms.uniform_(generator=self._numbers)
+        ops.sample_token(self.logits, self._uniforms, s.temperature, s.top_k, s.top_p, s.min_p, out=self.token)
 
     # -- the four entry points --------------------------------------------------
     # Prompts of at least this many rows run as dense blocks (tensor-core
@@ -181,6 +210,7 @@ class DecodeState:
             _lib.check(L.qb_prefill(self.engine.ctx, self.prompt.data_ptr(), n, self.token.data_ptr(),
                                     self.position.data_ptr(), _lib.ptr(self.logits), _lib.stream_handle()),
                        self.engine.ctx)
+        self._draw()
         return self.token
 
     def capture(self) -> None:
@@ -194,16 +224,18 @@ class DecodeState:
         self.captured = True
 
     def step(self) -> None:
-        """One decode step: token <- greedy(next), position += 1."""
+        """One decode step: token <- greedy(next), or drawn with ``sampling``; position += 1."""
         self._ensure_bound()
         if not self.captured:
             self.capture()
         _lib.check(_lib.load().qb_replay_decode(self.engine.ctx, _lib.stream_handle()), self.engine.ctx)
+        self._draw()
 
     def step_eager(self) -> None:
         self._ensure_bound()
         _lib.check(_lib.load().qb_decode_step(self.engine.ctx, self.token.data_ptr(), self.position.data_ptr(),
                                               _lib.ptr(self.logits), _lib.stream_handle()), self.engine.ctx)
+        self._draw()
 
     def read_token(self) -> List[int]:
         return self.token.tolist()
@@ -241,6 +273,8 @@ class DecodeState:
         self._ensure_bound()
         if self.batch > 1:
             raise ValueError("verify takes one sequence")
+        if self.sampling is not None:
+            raise ValueError("verify is greedy; it takes no sampling")
         n = len(proposal) + 1
         if n > 8:
             raise ValueError("verify takes at most 7 draft tokens")
@@ -351,8 +385,8 @@ class Engine:
         return self.state
 
     def generate(self, input_ids: List[List[int]], max_new_tokens: int, draft_tokens: Optional[int] = None,
-                 drafter=None):
-        """Greedy continuation; yields one token per sequence exactly
+                 drafter=None, sampling: Optional[Sampling] = None):
+        """Greedy continuation, or drawn tokens with ``sampling``; yields one token per sequence exactly
         ``max_new_tokens`` times (``dryft/engine/engine.py:202-249``).
 
         As in the reference, one sequence speculates by default: a
@@ -369,7 +403,16 @@ class Engine:
 
         Several sequences of equal prompt length decode together (every weight
         streamed once per step for up to 8 of them); more than 8 run as chunks
-        of 8, each on its own context over the same weights."""
+        of 8, each on its own context over the same weights.
+
+        ``sampling`` (one GPU) draws every token by its settings and its seed;
+        verification is greedy, so it decodes without speculation."""
+        if sampling is not None:
+            if draft_tokens or drafter is not None:
+                raise ValueError("speculation verifies greedily: sampling takes no draft_tokens or drafter")
+            if self.tp_size > 1:
+                raise ValueError("sampling runs on one GPU")
+            draft_tokens = 0
         if max_new_tokens <= 0:
             return
         B = len(input_ids)
@@ -389,18 +432,27 @@ class Engine:
             yield from self._generate_speculative(prompts, max_new_tokens, draft_tokens, drafter)
             return
         if B > DecodeState.MAX_BATCH:
-            yield from self._generate_chunked(prompts, max_new_tokens)
+            yield from self._generate_chunked(prompts, max_new_tokens, sampling)
             return
         P = len(prompts[0])
         with torch.inference_mode():
             shape = (B, P, max_new_tokens)
-            if self.state is None or self.state.shape != shape or self._bound_state is not self.state:
-                self.new_state(P, max_new_tokens, batch=B)
-            state = self.state
+            state = self._sampled_state(self, shape, sampling, 0)
             ids = torch.tensor(prompts if B > 1 else prompts[0], dtype=torch.int64).pin_memory()
             state.prefill(ids.to(self.device, non_blocking=True))
             first = state.read_token()
             yield from stream_decode(state, first, max_new_tokens, depth=self.STREAM_DEPTH)
+
+    @staticmethod
+    def _sampled_state(owner, shape, sampling: Optional[Sampling], lane: int) -> DecodeState:
+        """The owner's state for (B, P, N), kept from the last call where it fits."""
+        B, P, N = shape
+        state = owner.state
+        if (state is None or state.shape != shape or owner._bound_state is not state
+                or (state.sampling is None) != (sampling is None)):
+            state = owner.new_state(P, N, batch=B, sampling=sampling)
+        state.set_sampling(sampling, lane)
+        return state
 
     def _lane(self, i: int) -> "_Lane":
         """Context i (>= 1) for chunk i of a large batch: its own qb context and
@@ -409,7 +461,7 @@ class Engine:
             self._lanes.append(_Lane(self))
         return self._lanes[i - 1]
 
-    def _generate_chunked(self, prompts: List[List[int]], max_new_tokens: int):
+    def _generate_chunked(self, prompts: List[List[int]], max_new_tokens: int, sampling: Optional[Sampling] = None):
         """More than 8 sequences: chunks of 8 (the last may be smaller), chunk 0
         on this engine and chunk i on lane i; every step replays each chunk's
         graph, then yields all tokens in sequence order."""
@@ -423,9 +475,7 @@ class Engine:
             for i, chunk in enumerate(chunks):
                 owner = self if i == 0 else self._lane(i)
                 shape = (len(chunk), P, max_new_tokens)
-                st = owner.state
-                if st is None or st.shape != shape or owner._bound_state is not st:
-                    st = owner.new_state(P, max_new_tokens, batch=len(chunk))
+                st = self._sampled_state(owner, shape, sampling, i)
                 ids = torch.tensor(chunk if len(chunk) > 1 else chunk[0], dtype=torch.int64).pin_memory()
                 st.prefill(ids.to(self.device, non_blocking=True))
                 states.append(st)

@@ -229,3 +229,182 @@ def test_shared_prefix_matches_formula(lens, hq, hkv, page, prefix):
         _check(bt, out)
         outs.append(out)
     assert torch.equal(*outs)
+
+
+def _fresh(bt):
+    """The result of a call on the current stream, checked later."""
+    from hackthenorth_b200 import ops
+
+    return ops.paged_attention(bt["q"], bt["k"], bt["v"], bt["table"], bt["q_start"], bt["kv_lens"],
+                               max_queries=max(n for n, _ in bt["lens"]))
+
+
+def test_calls_on_several_streams_overlap():
+    """Long calls of both kernels on three streams at once, each with data made on its own stream."""
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    cases = [[(1, 9000)] * 3, [(40, 3000), (1, 5000)], [(1, 12000), (1, 4)]]
+    batches = [make_batch(c, 32, 8, 64, 60 + i, DEV) for i, c in enumerate(cases)]
+    torch.cuda.synchronize()
+    outs = [[] for _ in streams]
+    for _ in range(4):
+        for s, bt, o in zip(streams, batches, outs):
+            with torch.cuda.stream(s):
+                o.append(_fresh(bt))
+    torch.cuda.synchronize()
+    for bt, o in zip(batches, outs):
+        ref, mag = attention64(bt)
+        for x in o:
+            assert torch.equal(x, o[0])
+        assert bool(((o[0].double() - ref).abs() <= attention_bound(ref, mag)).all())
+
+
+def test_graphs_follow_the_lengths_and_share_no_workspace():
+    """Two captured graphs replayed on two streams at once, then again with longer sequences."""
+    from hackthenorth_b200 import ops
+
+    batches = [make_batch([(1, 6000), (1, 900)], 32, 8, 32, 70, DEV), make_batch([(30, 4000)], 32, 8, 64, 71, DEV)]
+    for bt in batches:
+        _fresh(bt)
+    graphs, outs = [], []
+    side = torch.cuda.Stream()
+    for bt in batches:
+        g, out = torch.cuda.CUDAGraph(), torch.zeros_like(bt["q"])
+        with torch.cuda.graph(g, stream=side):
+            ops.paged_attention(bt["q"], bt["k"], bt["v"], bt["table"], bt["q_start"], bt["kv_lens"],
+                                max_queries=max(n for n, _ in bt["lens"]), out=out)
+        graphs.append(g)
+        outs.append(out)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for shorter in (0, 700):
+        for bt in batches:
+            bt["lens"] = [(n, kv - shorter) for n, kv in bt["lens"]]
+            bt["kv_lens"].copy_(torch.tensor([kv for _, kv in bt["lens"]], dtype=torch.int32))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for g, s in zip(graphs, streams):
+                with torch.cuda.stream(s):
+                    g.replay()
+        torch.cuda.synchronize()
+        for bt, out in zip(batches, outs):
+            ref, mag = attention64(bt)
+            assert bool(((out.double() - ref).abs() <= attention_bound(ref, mag)).all())
+    ops.check_device_errors(DEV)
+
+
+@pytest.mark.parametrize("what,message", [("page", "page id"), ("negative page", "page id"), ("length", "lie outside"),
+                                          ("rows", "lie outside"), ("queries", "lie outside")])
+@pytest.mark.parametrize("n", [1, 40])
+def test_numbers_out_of_range_are_reported_and_spoil_no_other_sequence(what, message, n):
+    """The kernels check every page id, length and row range before they use it."""
+    from hackthenorth_b200 import ops
+
+    bt = make_batch([(n, 200), (1, 150), (1, 90)], 16, 8, 16, 80, DEV)
+    ref, mag = attention64(bt)
+    kw = dict(max_queries=n)
+    if what == "page":
+        bt["table"][1, 4] = bt["k"].shape[0]
+    elif what == "negative page":
+        bt["table"][1, 4] = -5
+    elif what == "length":
+        bt["kv_lens"][1] = bt["table"].shape[1] * 16 + 1
+    elif what == "rows":
+        bt["q_start"][3] = bt["rows"] + 7
+    else:
+        kw = dict(max_queries=n)
+        bt["q_start"][1:] = torch.tensor([0, n + 1, n + 2], dtype=torch.int32)  # the second sequence has n + 1 rows
+    out = torch.zeros_like(bt["q"])
+    ops.paged_attention(bt["q"], bt["k"], bt["v"], bt["table"], bt["q_start"], bt["kv_lens"], out=out, **kw)
+    with pytest.raises(ValueError, match=message):
+        ops.check_device_errors(DEV)
+    ops.check_device_errors(DEV)
+    if what != "queries":
+        good = out[:n].double()
+        assert bool(((good - ref[:n]).abs() <= attention_bound(ref[:n], mag[:n])).all())
+    again = make_batch([(n, 200), (1, 150), (1, 90)], 16, 8, 16, 80, DEV)  # and the next call is whole
+    _check(again, _attend(again, max_queries=n))
+
+
+def test_append_reports_pages_and_positions_out_of_range():
+    from hackthenorth_b200 import ops
+
+    bt = make_batch([(2, 20), (1, 40)], 16, 8, 16, 81, DEV)
+    qkv = torch.randn(3, 32 * D, device=DEV).to(BF16)
+    cos, sin = _tables(64)
+    for spoil, message in ((lambda: bt["table"].index_put_((torch.tensor([0], device=DEV), torch.tensor([1], device=DEV)),
+                                                           torch.tensor(99, dtype=torch.int32, device=DEV)), "page id"),
+                           (lambda: bt["kv_lens"].fill_(1), "KV capacity"), (lambda: bt["kv_lens"].fill_(1 << 20), "lie outside")):
+        table, lens = bt["table"].clone(), bt["kv_lens"].clone()
+        spoil()
+        k, v = bt["k"].clone(), bt["v"].clone()
+        ops.rope_paged_append(qkv, None, None, cos, sin, k, v, bt["table"], bt["q_start"], bt["kv_lens"])
+        with pytest.raises(ValueError, match=message):
+            ops.check_device_errors(DEV)
+        bt["table"], bt["kv_lens"] = table, lens
+    with_table = ops.rope_paged_append(qkv, None, None, cos[:30].contiguous(), sin[:30].contiguous(), bt["k"].clone(),
+                                       bt["v"].clone(), bt["table"], bt["q_start"], bt["kv_lens"])  # position 39 of 30 rows
+    assert with_table.shape == (3, 16, D)
+    with pytest.raises(ValueError, match="KV capacity"):
+        ops.check_device_errors(DEV)
+
+
+def test_pools_beyond_32_bits():
+    """Page ids whose elements lie past 2^32 in the pool."""
+    from hackthenorth_b200 import ops
+
+    pages, hkv, page = 70000, 8, 64  # 4.6e9 elements a pool
+    k = torch.empty(pages, hkv, page, D, dtype=BF16, device=DEV)
+    v = torch.empty_like(k)
+    ids = torch.tensor([69999, 3, 65536, 69998], dtype=torch.int32, device=DEV)
+    g = torch.Generator(device=DEV).manual_seed(1)
+    for i in ids.tolist():
+        k[i] = torch.randn(hkv, page, D, generator=g, device=DEV).to(BF16)
+        v[i] = torch.randn(hkv, page, D, generator=g, device=DEV).to(BF16)
+    lens = [(1, 250)]
+    for n in (1, 20):
+        bt = dict(lens=[(n, 250)], hq=32, hkv=hkv, page=page, starts=[0, n], rows=n, prefix=0, prefix_table=ids[:0],
+                  q=torch.randn(n, 32, D, generator=g, device=DEV).to(BF16), k=k, v=v, table=ids[None].contiguous(),
+                  pages=ids[None], q_start=torch.tensor([0, n], dtype=torch.int32, device=DEV),
+                  kv_lens=torch.tensor([250], dtype=torch.int32, device=DEV))
+        _check(bt, _attend(bt, max_queries=n))
+    qkv = torch.randn(1, 48 * D, generator=g, device=DEV).to(BF16)
+    cos, sin = _tables(256)
+    ops.rope_paged_append(qkv, None, None, cos, sin, k, v, ids[None].contiguous(), bt["q_start"] // 20, bt["kv_lens"])
+    ops.check_device_errors(DEV)
+    assert torch.equal(v[69998, :, 249 - 192], qkv.view(48, D)[40:])
+
+
+def test_serving_steps_match_the_contiguous_operators():
+    """Prompt appended and attended in one chunk, then single tokens, on pages:
+    as ``rope_attention`` and ``grouped_attention`` on a contiguous cache, and a
+    second sequence that shares the prompt as a prefix; the last row's token drawn."""
+    from hackthenorth_b200 import ops
+
+    hq, hkv, page, prompt, steps = 32, 8, 32, 75, 4
+    g = torch.Generator(device=DEV).manual_seed(90)
+    rnd = lambda *s: torch.randn(*s, generator=g, device=DEV).to(BF16)
+    rows = rnd(prompt + steps, (hq + 2 * hkv) * D)
+    qn, kn = (1 + 0.1 * torch.randn(2, D, generator=g, device=DEV)).to(BF16)
+    cos, sin = _tables(128)
+    kc, vc = (torch.zeros(hkv, 128, D, dtype=BF16, device=DEV) for _ in range(2))
+    want = [ops.rope_attention(rows[p], qn, kn, cos, sin, kc, vc, torch.tensor([p], device=DEV), n_heads=hq)
+            for p in range(prompt + steps)]
+    k, v = (torch.full((12, hkv, page, D), float("nan"), dtype=BF16, device=DEV) for _ in range(2))
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32, device=DEV)
+    table = i32(7, 2, 9, 4)[None].contiguous()
+    q = ops.rope_paged_append(rows[:prompt].contiguous(), qn, kn, cos, sin, k, v, table, i32(0, prompt), i32(prompt))
+    got = list(ops.paged_attention(q, k, v, table, i32(0, prompt), i32(prompt)))
+    own = i32(0, 11)[None].contiguous()
+    for p in range(prompt, prompt + steps):
+        row = rows[p][None].contiguous()
+        q = ops.rope_paged_append(row, qn, kn, cos, sin, k, v, table, i32(0, 1), i32(p + 1))
+        got.append(ops.paged_attention(q, k, v, table, i32(0, 1), i32(p + 1))[0])
+        # the same token behind the prompt as a shared prefix, its own keys on other pages
+        q = ops.rope_paged_append(row, qn, kn, cos, sin, k, v, own, i32(0, 1), i32(p + 1 - prompt), first_position=prompt)
+        shared = ops.shared_prefix_attention(q, k, v, table[0], prompt, own, i32(0, 1), i32(p + 1 - prompt))[0]
+        # two results of the same rows: each within the bound of the exact one
+        assert ((shared.float() - got[-1].float()).abs().max() / got[-1].float().abs().max()).item() <= 2e-2
+    ops.check_device_errors(DEV)
+    for a, b in zip(got, want):  # the cache rows differ by bf16 ulps (products rounded or not), so the outputs do
+        assert ((a.float() - b.float()).abs().max() / b.float().abs().max()).item() <= 2e-2
+    token = ops.sample_token(got[-1].reshape(1, -1), torch.full((1,), 0.5, device=DEV), top_k=1)
+    assert int(token) == int(got[-1].float().argmax())
