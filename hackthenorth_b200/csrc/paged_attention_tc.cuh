@@ -4,24 +4,33 @@
 //
 // The formula and the masks are those of paged_decode.cuh. A unit is up to 256
 // query rows of one sequence (two M = 128 tiles of 128 / G tokens with the G
-// query heads of one KV head) against the 128-key tiles that some of its rows
+// query heads of one KV head) against the 64-key tiles that some of its rows
 // sees. As there, the units' tiles form one line which is cut evenly over the
-// CTAs (one per SM); a cut unit leaves (m, l, O) of its pieces in the
-// workspace, and paged_join_kernel joins them: with 256 rows a piece is 128 KB,
-// too much for one CTA to join behind the others.
+// CTAs (one per SM), a unit's own start and end counted as four tiles (without
+// that the CTAs with many short units of a causal prompt finished last: 716 us
+// for 8100 tokens of 32/8 heads, 508 us with it, 516 us with seven tiles). A cut
+// unit leaves (m, l, O) of its pieces in the workspace, and paged_join_kernel
+// joins them: with 256 rows a piece is 128 KB, too much for one CTA to join
+// behind the others.
 //
-// Bound by the tensor cores where every key tile meets 256 rows (512 MMA-cycles
-// each for S and P.V of a tile and M tile) and by the cache's bytes below that.
+// Bound, where every key tile meets 256 rows, by the softmax and the MMAs
+// together (about 2000 cycles a key tile; the MMAs alone take 1280: 384 for S,
+// whose operands come from shared memory, and 256 for P.V of each M tile), and
+// by the cache's bytes below that. 8100 prompt tokens: 1.06 PFLOP/s.
 //  * warp 0: TMA. Q tiles (3D map, 128-byte swizzle) and K and V tiles of
-//    32 KB, a box per page, into two slots each.
-//  * warps 1 and 3: the MMAs of M tile 0 and 1. S_t = Q_t . K^T into TMEM columns 128 t, and
-//    once tile t's softmax has put P_t (bf16) over the first half of S_t,
-//    O_t += P_t . V with P_t read from TMEM into columns 256 + 128 t. S_t of the
-//    next key tile follows P_t . V in issue order, which is the order of
-//    execution, so one M tile's softmax runs under the other's MMAs.
+//    16 KB, a box per page, into four slots each.
+//  * warps 1 and 3: the MMAs of M tile 0 and 1. S_t = Q_t . K^T goes to one of
+//    two buffers of 64 TMEM columns in turn, so that the softmax finds the next
+//    one ready; P_t (bf16) comes back over the first half of its S, and O_t +=
+//    P_t . V reads it from there into columns 256 + 128 t. S_t of the tile after
+//    next follows P_t . V into the same buffer: issue order is the order of
+//    execution.
 //  * warps 4-7 and 8-11: softmax of M tile 0 and 1, a thread per row. The
 //    reference maximum only moves when a row's maximum grows by more than 8 (P
 //    stays below 2^8 and keeps its relative precision), so O is seldom rescaled.
+//    Both groups tend to reach their exponentials together, so every third pair
+//    is computed on the FMA pipe (a cubic; 2^-13.7 beside P's rounding of 2^-9):
+//    748 us without it, 724, 716 and 726 us with every fourth, third and second.
 //  * warp 2: walks the CTA's pieces of units ahead of the others and hands them
 //    over through a ring of 4 (the lookups and divisions of a new piece took 3 us
 //    of every role's time when each made them itself); and waits for K and V on
@@ -79,9 +88,8 @@ __host__ inline size_t pt_smem_bytes(int max_units) {
 
 // The MMAs as the whole warp runs them: `lead` (one lane) issues. Kept free of
 // divergence, descriptors and addresses stay in uniform registers, which the
-// instruction takes its operands from; issued from a lane's branch, every
-// operand was moved there anew, and the 32 MMAs of a key tile took longer to
-// issue (5000 cycles) than to run (2048).
+// instruction takes its operands from; in a lane's own branch every operand is
+// moved there anew.
 __device__ __forceinline__ bool elect_lane() {
   uint32_t r;
   asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
@@ -502,8 +510,8 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       };
       while (more && made < kPtPieces) hand_over();
       // The gatekeeper waits for the K and V tiles that a step's MMAs read and
-      // joins P's barrier for them: the MMA warps' own waits took 280 cycles
-      // each even where nothing was to be waited for, a quarter of their time.
+      // joins P's barrier for them: an MMA warp's own waits take 280 cycles each
+      // even where nothing is to be waited for, a quarter of its step.
       int J = 0;
       uint32_t phase = 0;  // bit 2 t + buffer
       walk([&](const PtPiece& pc) {

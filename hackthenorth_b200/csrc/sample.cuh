@@ -809,22 +809,36 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     }
     const unsigned long long want = top_k > 0 ? 0ull : wanted(whole);
     if (top_k <= kSmWarps * C / 2) {
-      unsigned long long weigh[kTops];
+      // found by one warp: all sixteen at it would take the issue slots of the SM's other rows
+      if (warp == 0) {
+        unsigned border = 0u;
+        if (top_k > 0) {
+          for (int bit = 31; bit >= kLowBits; --bit) {
+            const unsigned c = border | 1u << bit;
+            unsigned v = 0u;
 #pragma unroll
-      for (int j = 0; j < kTops; ++j) {
-        const float x = sample_value((unsigned)(tops[j] >> 32));
-        weigh[j] = top_k > 0 ? 1ull : tops[j] != 0ull ? mass_of(weight(x, depth(x))) : 0ull;
+            for (int j = 0; j < kTops; ++j) v += (unsigned)(tops[j] >> 32) >= c;
+            if (__reduce_add_sync(0xffffffffu, v) >= (unsigned)top_k) border = c;
+          }
+        } else {
+          unsigned long long q[kTops];
+#pragma unroll
+          for (int j = 0; j < kTops; ++j) {
+            const float x = sample_value((unsigned)(tops[j] >> 32));
+            q[j] = tops[j] != 0ull ? mass_of(weight(x, depth(x))) : 0ull;
+          }
+          for (int bit = 31; bit >= kLowBits; --bit) {
+            const unsigned c = border | 1u << bit;
+            unsigned long long v = 0ull;
+#pragma unroll
+            for (int j = 0; j < kTops; ++j) v += (unsigned)(tops[j] >> 32) >= c ? q[j] : 0ull;
+            if (warp_sum64(v) >= want) border = c;
+          }
+        }
+        if (lane == 0) sh.scan_cnt[0] = border;
       }
-      const unsigned long long wish = top_k > 0 ? (unsigned long long)top_k : want;
-      auto over = [&](unsigned c) {  // count or mass of the maxima whose pattern is at least c
-        unsigned long long v = 0ull;
-#pragma unroll
-        for (int j = 0; j < kTops; ++j) v += (unsigned)(tops[j] >> 32) >= c ? weigh[j] : 0ull;
-        return top_k > 0 ? (unsigned long long)__reduce_add_sync(0xffffffffu, (unsigned)v) : warp_sum64(v);
-      };
-      unsigned border = 0u;
-      for (int bit = 31; bit >= kLowBits; --bit)
-        if (over(border | 1u << bit) >= wish) border |= 1u << bit;
+      __syncthreads();
+      const unsigned border = sh.scan_cnt[0];
       // every value at or above the border's pattern (its low bits lack where bf16 has none: not above the value)
       if (border != 0u && finish_in_list(sample_value(border), kSmBins, top_k > 0, whole)) return;
     }

@@ -110,7 +110,7 @@ cudaError_t launch_paged_tc(const CUtensorMap& q, const CUtensorMap& k, const CU
 int check_tiles(int tokens, int n_seqs, int G, int table_width, int page_size) {
   const long long units = tc_units(tokens, n_seqs, G);
   if (units > kPtMaxUnits) return set_err(nullptr, QB_ERR_UNSUPPORTED, "more than 4096 blocks of 256 query rows per KV head");
-  if (std::max((long long)n_seqs, units) * ((long long)table_width * page_size / kPdKeys + 2) > 0x7fffffffll)
+  if (std::max((long long)n_seqs, units) * ((long long)table_width * page_size / kPdKeys + 2 + kPtUnitCost) > 0x7fffffffll)
     return set_err(nullptr, QB_ERR_UNSUPPORTED, "more than 2^31 key tiles over all sequences");
   return QB_OK;
 }

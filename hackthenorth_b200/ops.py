@@ -221,6 +221,14 @@ def _workspace(device, stream: int, max_queries: int, hq: int, hkv: int, prefix_
     return buf, nbytes
 
 
+def _no_grad(*ts):
+    """These operators have no backward pass: refuse what would silently lose a gradient."""
+    if torch.is_grad_enabled():
+        for t in ts:
+            if t is not None and t.requires_grad:
+                raise ValueError("this operator has no backward pass: use them under torch.no_grad()")
+
+
 def _on(device):
     """Make ``device`` current for the call (the library launches there)."""
     return _SAME if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
@@ -269,6 +277,7 @@ def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_tabl
     from ``q_start[B]`` on are left as they are in ``out``. Page ids, lengths
     or positions out of range are skipped and raise in ``check_device_errors``.
     ``dryft/engine/kernels/fused.py:9-30,47-82`` for a ragged batch."""
+    _no_grad(qkv, q_norm, k_norm, k_pages, v_pages)
     _bf16_cuda(qkv, q_norm, k_norm, cos, sin)
     dev = qkv.device
     pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
@@ -280,13 +289,15 @@ def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_tabl
         _require(t is None or t.device == dev, "norms and rope tables must be on the device of qkv")
     for t in (q_norm, k_norm):
         _require(t is None or t.numel() == 128, "norm gains must have 128 entries")
+    first_position = int(first_position)
+    _require(0 <= first_position < 1 << 30, "first_position must lie in 0..2^30")
     tokens = qkv.shape[0]
     with _on(dev):
         out = _rows_out(out, (tokens, hq, 128), dev)
         _lib.check(_lib.load().qb_rope_paged_append(
             qkv.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), cos.data_ptr(), sin.data_ptr(), cos.shape[0], float(eps),
             k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width, q_start.data_ptr(),
-            kv_lens.data_ptr(), seqs, tokens, int(first_position), hq, hkv, out.data_ptr(), _status(dev),
+            kv_lens.data_ptr(), seqs, tokens, first_position, hq, hkv, out.data_ptr(), _status(dev),
             _raw_stream(dev.index)))
     return out
 
@@ -305,20 +316,22 @@ def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0,
     that is not finite in a key that one row of a sequence sees may reach that
     sequence's other rows. ``dryft/engine/kernels/attention.py:200-237`` for a
     ragged batch."""
+    _no_grad(q, k_pages, v_pages)
     _bf16_cuda(q)
     dev = q.device
     pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
     _require(q.dim() == 3 and q.shape[2] == 128 and q.shape[1] % hkv == 0, "expected q [T, Hq, 128], Hq a multiple of Hkv")
+    window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)  # beyond any sequence
+    _require(window >= 0 and sinks >= 0, "window and sinks must not be negative")
     tokens, hq = q.shape[:2]
-    if max_queries is None:
-        max_queries = tokens
+    max_queries = tokens if max_queries is None else min(int(max_queries), tokens)
     with _on(dev):
         out = _rows_out(out, q.shape, dev)
         stream = _raw_stream(dev.index)
         ws, need = _workspace(dev, stream, max_queries, hq, hkv, 0)
         _lib.check(_lib.load().qb_paged_attention(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
-            q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, int(max_queries), hq, hkv, int(window), int(sinks),
+            q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, max_queries, hq, hkv, window, sinks,
             out.data_ptr(), ws.data_ptr(), need, _status(dev), stream))
     return out
 
@@ -331,23 +344,25 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
     Each query sees the whole prefix and its sequence's own keys up to its
     position; ``kv_lens`` and ``page_table`` count and place the own keys only
     (append them with ``first_position=prefix_len``)."""
+    _no_grad(q, k_pages, v_pages)
     _bf16_cuda(q)
     dev = q.device
     pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
     _require(q.dim() == 3 and q.shape[2] == 128 and q.shape[1] % hkv == 0, "expected q [T, Hq, 128], Hq a multiple of Hkv")
+    prefix_len = int(prefix_len)
+    _require(0 <= prefix_len <= prefix_table.numel() * page, "prefix_len must lie in 0..prefix_table's keys")
     _require(prefix_table.dim() == 1 and prefix_table.dtype == torch.int32 and prefix_table.device == dev
              and prefix_table.is_contiguous(), "prefix_table must be a contiguous int32 tensor [n] on the device of q")
     tokens, hq = q.shape[:2]
-    if max_queries is None:
-        max_queries = tokens
+    max_queries = tokens if max_queries is None else min(int(max_queries), tokens)
     with _on(dev):
         out = _rows_out(out, q.shape, dev)
         stream = _raw_stream(dev.index)
         ws, need = _workspace(dev, stream, max_queries, hq, hkv, tokens)
         _lib.check(_lib.load().qb_shared_prefix_attention(
             q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, prefix_table.data_ptr(),
-            prefix_table.shape[0], int(prefix_len), page_table.data_ptr(), width, q_start.data_ptr(),
-            kv_lens.data_ptr(), seqs, tokens, int(max_queries), hq, hkv, out.data_ptr(), ws.data_ptr(), need,
+            prefix_table.shape[0], prefix_len, page_table.data_ptr(), width, q_start.data_ptr(),
+            kv_lens.data_ptr(), seqs, tokens, max_queries, hq, hkv, out.data_ptr(), ws.data_ptr(), need,
             _status(dev), stream))
     return out
 
@@ -376,6 +391,7 @@ def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     ``greedy_token``. A row without a finite logit gives -1 and raises in
     ``check_device_errors``. The sampled counterpart of
     ``dryft/engine/kernels/greedy.py:45-60``."""
+    _no_grad(logits)
     _require(logits.is_cuda and logits.dtype in (BF16, torch.float32) and logits.is_contiguous() and logits.dim() in (1, 2),
              "expected contiguous bf16 or fp32 CUDA logits [R, V]")
     dev, vocab = logits.device, logits.shape[-1]

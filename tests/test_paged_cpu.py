@@ -68,6 +68,16 @@ def test_sizes_beyond_the_tile_counts_are_refused(built_lib):
     assert _attention(built_lib, seqs=1024, width=1 << 26) == UNSUPPORTED  # too many key tiles
 
 
+def test_tensors_that_require_a_gradient_are_refused():
+    from hackthenorth_b200 import ops
+
+    q = torch.zeros(1, 16, 128, dtype=torch.bfloat16, requires_grad=True)
+    for call in (lambda: ops.paged_attention(q, q, q, q, q, q), lambda: ops.shared_prefix_attention(q, q, q, q, 0, q, q, q),
+                 lambda: ops.rope_paged_append(q, q, q, q, q, q, q, q, q, q), lambda: ops.sample_token(q, q)):
+        with pytest.raises(ValueError, match="backward"):
+            call()
+
+
 def test_empty_calls_return_without_a_launch(built_lib):
     assert _append(built_lib, tokens=0, qkv=None, out=None) == 0
     assert _attention(built_lib, tokens=0, q=None, out=None) == 0
