@@ -37,7 +37,7 @@ constexpr int kPdThreads = (kPdWarps + 1) * 32;
 constexpr int kPdStageBytes = 4 * kAttnSubTile;  // K lo, K hi, V lo, V hi
 constexpr int kPdPStride = kPdKeys * 2 + 16;     // bytes of a P row; 16 more keep ldmatrix free of conflicts
 constexpr int kPdCtasPerSm = 2;
-constexpr int kPdMinTiles = 2;                   // fewest tiles worth a CTA of their own
+constexpr int kPdMinTiles = 1;                   // fewest tiles of a CTA: 1 of 16 in 24 us, 2 in 29, 4 in 40 (six short rows)
 
 // Where a finished row goes: out (bf16), or out32 / lse32 (normalised fp32 and
 // log-sum-exp in base 2, for a later join); base32 / base_lse: a part of the

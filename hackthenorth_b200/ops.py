@@ -186,6 +186,7 @@ def rope_attention(qkv, q_norm, k_norm, cos, sin, keys, values, position, eps=1e
 I32 = torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
     lambda index: torch.cuda.current_stream(index).cuda_stream)
+_capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_current_stream_capturing)
 _workspace_bytes = {}
 
 
@@ -209,7 +210,7 @@ def _workspace(device, stream: int, max_queries: int, hq: int, hkv: int, prefix_
         if len(_workspace_bytes) > 4096:
             _workspace_bytes.clear()
         nbytes = _workspace_bytes[key] = n.value
-    if torch.cuda.is_current_stream_capturing():
+    if _capturing():
         buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
         buf[:8192].zero_()  # qb_paged_zero_bytes()
         return buf, nbytes
@@ -242,13 +243,14 @@ def _batch(device, k_pages, v_pages, page_table, q_start, kv_lens):
     shape = k_pages.shape
     if len(shape) != 4 or shape[3] != 128 or v_pages.shape != shape:
         raise ValueError("expected k_pages and v_pages [pages, Hkv, page, 128]")
-    if not (k_pages.dtype == BF16 and v_pages.dtype == BF16 and k_pages.is_contiguous() and v_pages.is_contiguous()
-            and k_pages.device == device and v_pages.device == device):
-        raise ValueError("expected contiguous bf16 pools on the device of the queries")
-    if not (page_table.dtype == I32 and q_start.dtype == I32 and kv_lens.dtype == I32 and page_table.is_contiguous()
-            and q_start.is_contiguous() and kv_lens.is_contiguous() and page_table.device == device
-            and q_start.device == device and kv_lens.device == device):
-        raise ValueError("page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the queries")
+    i = device.index
+    for t in (k_pages, v_pages):
+        if t.dtype is not BF16 or t.get_device() != i or not t.is_contiguous():
+            raise ValueError("expected contiguous bf16 pools on the device of the queries")
+    for t in (page_table, q_start, kv_lens):
+        if t.dtype is not I32 or t.get_device() != i or not t.is_contiguous():
+            raise ValueError("page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the "
+                             "queries")
     table, seqs = page_table.shape, kv_lens.shape
     if len(table) != 2 or len(seqs) != 1 or table[0] != seqs[0] or q_start.shape != (seqs[0] + 1,):
         raise ValueError("expected page_table [B, P], q_start [B + 1], kv_lens [B]")
@@ -258,7 +260,7 @@ def _batch(device, k_pages, v_pages, page_table, q_start, kv_lens):
 def _rows_out(out, shape, device):
     if out is None:
         return torch.empty(shape, dtype=BF16, device=device)
-    if not (out.dtype == BF16 and out.device == device and out.is_contiguous() and out.shape == shape):
+    if out.dtype is not BF16 or out.get_device() != device.index or not out.is_contiguous() or out.shape != shape:
         raise ValueError("out must be a contiguous bf16 tensor of the result's shape on the device of the queries")
     return out
 
