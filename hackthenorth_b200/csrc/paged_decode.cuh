@@ -39,6 +39,8 @@ constexpr int kPdPStride = kPdKeys * 2 + 16;     // bytes of a P row; 16 more ke
 constexpr int kPdCtasPerSm = 2;
 constexpr int kPdMinTiles = 1;                   // fewest tiles of a CTA: 1 of 16 in 24 us, 2 in 29, 4 in 40 (six short rows)
 
+constexpr int kPdUnitCost = 2;  // what beginning and ending a unit takes, in key tiles: its place in the line
+
 // Where a finished row goes: out (bf16), or out32 / lse32 (normalised fp32 and
 // log-sum-exp in base 2, for a later join); base32 / base_lse: a part of the
 // row's keys already attended to, joined in.
@@ -107,6 +109,16 @@ __host__ inline size_t pd_smem_bytes() {
          2 * kPdStages * 8 + 64 + (kPagedMaxSeqs + 1) * 4 + 4 + kPagedMaxSeqs * 8;
 }
 
+// Sum of v over the block.
+__device__ __forceinline__ int block_count(int v, int* warp_tot) {
+  v = __reduce_add_sync(0xffffffffu, v);
+  if ((threadIdx.x & 31) == 0) warp_tot[threadIdx.x >> 5] = v;
+  __syncthreads();
+  int all = 0;
+  for (int w = 0; w < (int)blockDim.x / 32; ++w) all += warp_tot[w];
+  return all;
+}
+
 __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
     paged_decode_kernel(const __grid_constant__ CUtensorMap tmk, const __grid_constant__ CUtensorMap tmv,
                         const PagedAttnArgs a) {
@@ -138,14 +150,17 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
   pdl_trigger();
 
   // Tiles of every sequence, summed up (each CTA for itself).
-  int carry = 0;
+  int carry = 0, live = 0;  // live: this thread's sequences with rows
   for (int s0 = 0; s0 < b.n_seqs; s0 += kPdThreads) {
     const int s = s0 + threadIdx.x;
     int cnt = 0;
     if (s < b.n_seqs) {
       const SeqSpan sp = paged_seq(b, s, a.err);
       seqs[s] = make_int2(sp.q0 | sp.n << 25, sp.kv);
-      if (sp.n > 0) cnt = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks).count;
+      if (sp.n > 0) {
+        cnt = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks).count + kPdUnitCost;
+        ++live;
+      }
     }
     int v = cnt;
 #pragma unroll
@@ -169,7 +184,8 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
   __syncthreads();
 
   const long long total = (long long)carry * a.Hkv;
-  const int E = (int)min((long long)gridDim.x, max(1ll, total / kPdMinTiles));
+  const int tiles = carry - kPdUnitCost * block_count(live, warp_tot);
+  const int E = (int)min((long long)gridDim.x, max(1ll, (long long)tiles * a.Hkv / kPdMinTiles));
   const int me = blockIdx.x;
   if (me >= E || total == 0) return;
   const long long t_begin = tile_begin(me, total, E), t_end = tile_begin(me + 1, total, E);
@@ -193,12 +209,12 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
     bool ok = true;
     int seq = seq0;
     for (long long t = t_begin; t < t_end && ok; ++seq) {
-      const int n_tiles = pref[seq + 1] - pref[seq];
-      if (n_tiles == 0) continue;
+      const int places = pref[seq + 1] - pref[seq];  // of one head in the line
+      if (places == 0) continue;
       const SeqSpan sp = {seqs[seq].x & 0x1ffffff, seqs[seq].x >> 25, seqs[seq].y};
       const TileSpan ts = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks);
       const long long base = (long long)pref[seq] * a.Hkv;
-      const long long stop = min(t_end, base + (long long)n_tiles * a.Hkv);
+      const long long stop = min(t_end, base + (long long)places * a.Hkv);
       // page of this lane's box of the tile at k, or -1
       auto page_of = [&](int k) {
         const int c0 = (k < ts.n_sink ? k : k - ts.n_sink + ts.lo_tile) * kPdKeys + box * br;
@@ -210,27 +226,31 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
         }
         return page;
       };
-      int k = (int)((t - base) % n_tiles);
+      int k = max(0, (int)((t - base) % places) - kPdUnitCost);
       int page = page_of(k);
-      for (; t < stop && ok; ++t) {
-        const int g = (int)((t - base) / n_tiles);
-        const int c0 = (k < ts.n_sink ? k : k - ts.n_sink + ts.lo_tile) * kPdKeys + box * br;
-        const int s = issued % kPdStages;
-        const int now = page;
-        k = k + 1 == n_tiles ? 0 : k + 1;
-        page = page_of(k);  // its load runs while the slot is waited for
-        if (issued >= kPdStages)
-          ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((issued / kPdStages) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY));
-        if (!ok) break;
-        const uint32_t need = __ballot_sync(0xffffffffu, now >= 0);
-        if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)__popc(need) * br * 128);
-        __syncwarp();
-        if (now >= 0) {
-          const int y = ((now * a.Hkv + g) << b.page_log2) + (c0 & ((1 << b.page_log2) - 1));
-          tma_load_2d(ring + s * kPdStageBytes + kind * kAttnSubTile + box * br * 128, kind < 2 ? &tmk : &tmv,
-                      64 * (kind & 1), y, &full[s]);
+      while (t < stop && ok) {
+        const int g = (int)((t - base) / places);
+        const int x0 = (int)(t - base - (long long)g * places), x1 = (int)min((long long)places, x0 + (t_end - t));
+        const int k1 = max(0, x1 - kPdUnitCost);
+        for (k = max(0, x0 - kPdUnitCost); k < k1; ++k) {
+          const int c0 = (k < ts.n_sink ? k : k - ts.n_sink + ts.lo_tile) * kPdKeys + box * br;
+          const int s = issued % kPdStages;
+          const int now = page;
+          page = page_of(k + 1 == places - kPdUnitCost ? 0 : k + 1);  // its load runs while the slot is waited for
+          if (issued >= kPdStages)
+            ok = __all_sync(0xffffffffu, mbar_wait(&empty[s], ((issued / kPdStages) - 1) & 1, a.err, DEV_TIMEOUT_ATTN_EMPTY));
+          if (!ok) break;
+          const uint32_t need = __ballot_sync(0xffffffffu, now >= 0);
+          if (lane == 0) mbar_arrive_expect_tx(&full[s], (uint32_t)__popc(need) * br * 128);
+          __syncwarp();
+          if (now >= 0) {
+            const int y = ((now * a.Hkv + g) << b.page_log2) + (c0 & ((1 << b.page_log2) - 1));
+            tma_load_2d(ring + s * kPdStageBytes + kind * kAttnSubTile + box * br * 128, kind < 2 ? &tmk : &tmv,
+                        64 * (kind & 1), y, &full[s]);
+          }
+          ++issued;
         }
-        ++issued;
+        t += x1 - x0;
       }
     }
     // keep shared memory alive until every issued copy has landed
@@ -244,21 +264,26 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
   int used = 0;
   int seq = seq0;
   for (long long t = t_begin; t < t_end; ++seq) {
-    const int n_tiles = pref[seq + 1] - pref[seq];
-    if (n_tiles == 0) continue;
+    const int places = pref[seq + 1] - pref[seq], n_tiles = places - kPdUnitCost;
+    if (places == 0) continue;
     const SeqSpan sp = {seqs[seq].x & 0x1ffffff, seqs[seq].x >> 25, seqs[seq].y};
     const TileSpan ts = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks);
     const long long base = (long long)pref[seq] * a.Hkv;
-    const long long stop = min(t_end, base + (long long)n_tiles * a.Hkv);
+    const long long stop = min(t_end, base + (long long)places * a.Hkv);
     const int rows = sp.n * a.G;
     int pos[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) pos[h] = r_lo + 8 * h < rows ? sp.kv - sp.n + (r_lo + 8 * h) / a.G : -1;
     const int p_first = sp.kv - sp.n;
     while (t < stop) {
-      const int g = (int)((t - base) / n_tiles);
-      const long long u0 = base + (long long)g * n_tiles;  // the unit's first tile
-      const int k0 = (int)(t - u0), k1 = (int)min((long long)n_tiles, (long long)k0 + (t_end - t));
+      const int g = (int)((t - base) / places);
+      const long long u0 = base + (long long)g * places;  // the unit's place in the line: first those without a tile
+      const int x0 = (int)(t - u0), x1 = (int)min((long long)places, x0 + (t_end - t));
+      const int k0 = max(0, x0 - kPdUnitCost), k1 = max(0, x1 - kPdUnitCost);
+      if (k0 == k1) {
+        t += x1 - x0;
+        continue;
+      }
       // Q as the MMA's A operand, straight from memory
       uint32_t qa[8][4];
 #pragma unroll
@@ -418,7 +443,7 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
         }
       }
       if (!whole) {
-        const int cf = tile_owner(u0, total, E), cl = tile_owner(u0 + n_tiles - 1, total, E);
+        const int cf = tile_owner(u0 + kPdUnitCost, total, E), cl = tile_owner(u0 + places - 1, total, E);
         named_barrier(1, kPdWarps * 32);
         if (threadIdx.x == 0) {
           const unsigned old = atomic_add_acq_rel_gpu(&a.tickets[cf], 1u);
@@ -468,7 +493,7 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
           }
         }
       }
-      t += k1 - k0;
+      t += x1 - x0;
     }
   }
 }
