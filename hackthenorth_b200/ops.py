@@ -8,8 +8,6 @@ the CUDA library; there is no PyTorch or CPU fallback.
 """
 from __future__ import annotations
 
-import contextlib
-
 import torch
 
 from . import _lib
@@ -190,19 +188,22 @@ _capturing = getattr(torch._C, "_cuda_isCurrentStreamCapturing", torch.cuda.is_c
 _workspace_bytes = {}
 
 
-def _status(device) -> int:
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+
+
+def _status(index: int) -> int:
     """Address of the device error word that ``check_device_errors`` reads."""
-    buf = _scratch.get(device.index)
+    buf = _scratch.get(index)
     if buf is None:
         if torch.cuda.is_current_stream_capturing():
             raise RuntimeError("call an operator once on this device before capturing a graph")
-        buf = _op_scratch(device)
+        buf = _op_scratch(torch.device("cuda", index))
     return buf.data_ptr()
 
 
-def _workspace(device, stream: int, max_queries: int, hq: int, hkv: int, prefix_tokens: int):
+def _workspace(index: int, stream: int, max_queries: int, hq: int, hkv: int, prefix_tokens: int):
     """Workspace of a paged call: (the tensor, its size in bytes)."""
-    key = (device.index, max_queries, hq, hkv, prefix_tokens)
+    key = (index, max_queries, hq, hkv, prefix_tokens)
     nbytes = _workspace_bytes.get(key)
     if nbytes is None:
         n = _lib.c_size_t()
@@ -210,15 +211,13 @@ def _workspace(device, stream: int, max_queries: int, hq: int, hkv: int, prefix_
         if len(_workspace_bytes) > 4096:
             _workspace_bytes.clear()
         nbytes = _workspace_bytes[key] = n.value
-    if _capturing():
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        buf[:8192].zero_()  # qb_paged_zero_bytes()
-        return buf, nbytes
-    buf = _workspaces.get((device.index, stream))
+    captured = _capturing()
+    buf = None if captured else _workspaces.get((index, stream))
     if buf is None or buf.numel() < nbytes:
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=device)
-        buf[:8192].zero_()
-        _workspaces[device.index, stream] = buf
+        buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+        buf[:8192].zero_()  # qb_paged_zero_bytes()
+        if not captured:
+            _workspaces[index, stream] = buf
     return buf, nbytes
 
 
@@ -227,42 +226,46 @@ def _no_grad(*ts):
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
-                raise ValueError("this operator has no backward pass: use them under torch.no_grad()")
+                raise ValueError("this operator has no backward pass: use it under torch.no_grad()")
 
 
-def _on(device):
-    """Make ``device`` current for the call (the library launches there)."""
-    return _SAME if torch._C._cuda_getDevice() == device.index else torch.cuda.device(device)
+def _is_bf16(t, index: int) -> bool:
+    return t.dtype is BF16 and t.get_device() == index and t.is_contiguous()
 
 
-_SAME = contextlib.nullcontext()
+def _is_i32(t, index: int) -> bool:
+    return t.dtype is I32 and t.get_device() == index and t.is_contiguous()
 
 
-def _batch(device, k_pages, v_pages, page_table, q_start, kv_lens):
+def _batch(index: int, k_pages, v_pages, page_table, q_start, kv_lens):
     """Checked (pages, Hkv, page, table width, sequences) of a paged batch."""
-    shape = k_pages.shape
-    if len(shape) != 4 or shape[3] != 128 or v_pages.shape != shape:
+    shape, table, seqs = k_pages.shape, page_table.shape, kv_lens.shape
+    if len(shape) != 4 or shape[3] != 128 or shape[1] < 1 or v_pages.shape != shape:
         raise ValueError("expected k_pages and v_pages [pages, Hkv, page, 128]")
-    i = device.index
-    for t in (k_pages, v_pages):
-        if t.dtype is not BF16 or t.get_device() != i or not t.is_contiguous():
-            raise ValueError("expected contiguous bf16 pools on the device of the queries")
-    for t in (page_table, q_start, kv_lens):
-        if t.dtype is not I32 or t.get_device() != i or not t.is_contiguous():
-            raise ValueError("page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the "
-                             "queries")
-    table, seqs = page_table.shape, kv_lens.shape
+    if index < 0 or not (_is_bf16(k_pages, index) and _is_bf16(v_pages, index)):
+        raise ValueError("expected contiguous bf16 pools on the device of the queries")
+    if not (_is_i32(page_table, index) and _is_i32(q_start, index) and _is_i32(kv_lens, index)):
+        raise ValueError("page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the queries")
     if len(table) != 2 or len(seqs) != 1 or table[0] != seqs[0] or q_start.shape != (seqs[0] + 1,):
         raise ValueError("expected page_table [B, P], q_start [B + 1], kv_lens [B]")
     return shape[0], shape[1], shape[2], table[1], seqs[0]
 
 
-def _rows_out(out, shape, device):
+def _rows_out(out, shape, like):
     if out is None:
-        return torch.empty(shape, dtype=BF16, device=device)
-    if out.dtype is not BF16 or out.get_device() != device.index or not out.is_contiguous() or out.shape != shape:
+        return torch.empty(shape, dtype=BF16, device=like.device)
+    if not _is_bf16(out, like.get_device()) or out.shape != shape:
         raise ValueError("out must be a contiguous bf16 tensor of the result's shape on the device of the queries")
     return out
+
+
+def _queries(q, hkv: int, index: int, max_queries):
+    """Checked (rows, query heads, bound of a sequence's rows)."""
+    shape = q.shape
+    if not _is_bf16(q, index) or len(shape) != 3 or shape[2] != 128 or shape[1] < 1 or shape[1] % hkv:
+        raise ValueError("expected contiguous bf16 CUDA queries [T, Hq, 128], Hq a multiple of Hkv")
+    tokens = shape[0]
+    return tokens, shape[1], tokens if max_queries is None else min(int(max_queries), tokens)
 
 
 def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_table, q_start, kv_lens, eps=1e-6,
@@ -280,27 +283,34 @@ def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_tabl
     or positions out of range are skipped and raise in ``check_device_errors``.
     ``dryft/engine/kernels/fused.py:9-30,47-82`` for a ragged batch."""
     _no_grad(qkv, q_norm, k_norm, k_pages, v_pages)
-    _bf16_cuda(qkv, q_norm, k_norm, cos, sin)
-    dev = qkv.device
-    pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
-    _require(qkv.dim() == 2 and qkv.shape[1] % 128 == 0, "expected qkv [T, (Hq + 2 Hkv) 128]")
-    hq = n_heads if n_heads is not None else qkv.shape[1] // 128 - 2 * hkv
-    _require(hq > 0 and qkv.shape[1] == (hq + 2 * hkv) * 128, "packed qkv width does not match the cache heads")
-    _require(cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] == 128, "expected cos and sin [positions, 128]")
-    for t in (q_norm, k_norm, cos, sin):
-        _require(t is None or t.device == dev, "norms and rope tables must be on the device of qkv")
-    for t in (q_norm, k_norm):
-        _require(t is None or t.numel() == 128, "norm gains must have 128 entries")
-    first_position = int(first_position)
-    _require(0 <= first_position < 1 << 30, "first_position must lie in 0..2^30")
-    tokens = qkv.shape[0]
-    with _on(dev):
-        out = _rows_out(out, (tokens, hq, 128), dev)
-        _lib.check(_lib.load().qb_rope_paged_append(
-            qkv.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), cos.data_ptr(), sin.data_ptr(), cos.shape[0], float(eps),
-            k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width, q_start.data_ptr(),
-            kv_lens.data_ptr(), seqs, tokens, first_position, hq, hkv, out.data_ptr(), _status(dev),
-            _raw_stream(dev.index)))
+    index = qkv.get_device()
+    if not (_is_bf16(qkv, index) and _is_bf16(cos, index) and _is_bf16(sin, index)
+            and (q_norm is None or _is_bf16(q_norm, index)) and (k_norm is None or _is_bf16(k_norm, index))):
+        raise ValueError("expected contiguous bf16 CUDA tensors on one device")
+    pages, hkv, page, width, seqs = _batch(index, k_pages, v_pages, page_table, q_start, kv_lens)
+    rows, table = qkv.shape, cos.shape
+    if len(rows) != 2 or rows[1] % 128:
+        raise ValueError("expected qkv [T, (Hq + 2 Hkv) 128]")
+    hq = n_heads if n_heads is not None else rows[1] // 128 - 2 * hkv
+    if hq < 1 or rows[1] != (hq + 2 * hkv) * 128:
+        raise ValueError("packed qkv width does not match the cache heads")
+    if len(table) != 2 or table[1] != 128 or sin.shape != table:
+        raise ValueError("expected cos and sin [positions, 128]")
+    if (q_norm is not None and q_norm.numel() != 128) or (k_norm is not None and k_norm.numel() != 128):
+        raise ValueError("norm gains must have 128 entries")
+    if not 0 <= first_position < 1 << 30:
+        raise ValueError("first_position must lie in 0..2^30")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_table, q_start, kv_lens, eps,
+                                     n_heads, first_position, out)
+    out = _rows_out(out, (rows[0], hq, 128), qkv)
+    rc = _lib.load().qb_rope_paged_append(
+        qkv.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), cos.data_ptr(), sin.data_ptr(), table[0], eps,
+        k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width, q_start.data_ptr(),
+        kv_lens.data_ptr(), seqs, rows[0], first_position, hq, hkv, out.data_ptr(), _status(index), _raw_stream(index))
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -319,22 +329,24 @@ def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0,
     sequence's other rows. ``dryft/engine/kernels/attention.py:200-237`` for a
     ragged batch."""
     _no_grad(q, k_pages, v_pages)
-    _bf16_cuda(q)
-    dev = q.device
-    pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
-    _require(q.dim() == 3 and q.shape[2] == 128 and q.shape[1] % hkv == 0, "expected q [T, Hq, 128], Hq a multiple of Hkv")
+    index = q.get_device()
+    pages, hkv, page, width, seqs = _batch(index, k_pages, v_pages, page_table, q_start, kv_lens)
+    tokens, hq, max_queries = _queries(q, hkv, index, max_queries)
     window, sinks = min(int(window), 1 << 30), min(int(sinks), 1 << 30)  # beyond any sequence
-    _require(window >= 0 and sinks >= 0, "window and sinks must not be negative")
-    tokens, hq = q.shape[:2]
-    max_queries = tokens if max_queries is None else min(int(max_queries), tokens)
-    with _on(dev):
-        out = _rows_out(out, q.shape, dev)
-        stream = _raw_stream(dev.index)
-        ws, need = _workspace(dev, stream, max_queries, hq, hkv, 0)
-        _lib.check(_lib.load().qb_paged_attention(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
-            q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, max_queries, hq, hkv, window, sinks,
-            out.data_ptr(), ws.data_ptr(), need, _status(dev), stream))
+    if window < 0 or sinks < 0:
+        raise ValueError("window and sinks must not be negative")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window, sinks, max_queries, out)
+    out = _rows_out(out, q.shape, q)
+    stream = _raw_stream(index)
+    ws, need = _workspace(index, stream, max_queries, hq, hkv, 0)
+    rc = _lib.load().qb_paged_attention(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
+        q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, max_queries, hq, hkv, window, sinks, out.data_ptr(),
+        ws.data_ptr(), need, _status(index), stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
@@ -347,35 +359,37 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
     position; ``kv_lens`` and ``page_table`` count and place the own keys only
     (append them with ``first_position=prefix_len``)."""
     _no_grad(q, k_pages, v_pages)
-    _bf16_cuda(q)
-    dev = q.device
-    pages, hkv, page, width, seqs = _batch(dev, k_pages, v_pages, page_table, q_start, kv_lens)
-    _require(q.dim() == 3 and q.shape[2] == 128 and q.shape[1] % hkv == 0, "expected q [T, Hq, 128], Hq a multiple of Hkv")
-    prefix_len = int(prefix_len)
-    _require(0 <= prefix_len <= prefix_table.numel() * page, "prefix_len must lie in 0..prefix_table's keys")
-    _require(prefix_table.dim() == 1 and prefix_table.dtype == torch.int32 and prefix_table.device == dev
-             and prefix_table.is_contiguous(), "prefix_table must be a contiguous int32 tensor [n] on the device of q")
-    tokens, hq = q.shape[:2]
-    max_queries = tokens if max_queries is None else min(int(max_queries), tokens)
-    with _on(dev):
-        out = _rows_out(out, q.shape, dev)
-        stream = _raw_stream(dev.index)
-        ws, need = _workspace(dev, stream, max_queries, hq, hkv, tokens)
-        _lib.check(_lib.load().qb_shared_prefix_attention(
-            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, prefix_table.data_ptr(),
-            prefix_table.shape[0], prefix_len, page_table.data_ptr(), width, q_start.data_ptr(),
-            kv_lens.data_ptr(), seqs, tokens, max_queries, hq, hkv, out.data_ptr(), ws.data_ptr(), need,
-            _status(dev), stream))
+    index = q.get_device()
+    pages, hkv, page, width, seqs = _batch(index, k_pages, v_pages, page_table, q_start, kv_lens)
+    tokens, hq, max_queries = _queries(q, hkv, index, max_queries)
+    if not _is_i32(prefix_table, index) or prefix_table.dim() != 1:
+        raise ValueError("prefix_table must be a contiguous int32 tensor [n] on the device of q")
+    if not 0 <= prefix_len <= prefix_table.numel() * page:
+        raise ValueError("prefix_len must lie in 0..prefix_table's keys")
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_table, q_start, kv_lens,
+                                           max_queries, out)
+    out = _rows_out(out, q.shape, q)
+    stream = _raw_stream(index)
+    ws, need = _workspace(index, stream, max_queries, hq, hkv, tokens)
+    rc = _lib.load().qb_shared_prefix_attention(
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, prefix_table.data_ptr(),
+        prefix_table.shape[0], prefix_len, page_table.data_ptr(), width, q_start.data_ptr(), kv_lens.data_ptr(), seqs,
+        tokens, max_queries, hq, hkv, out.data_ptr(), ws.data_ptr(), need, _status(index), stream)
+    if rc:
+        _lib.check(rc)
     return out
 
 
-def _setting(value, name, rows, dtype, device, lo, hi):
+def _setting(value, name, rows, dtype, index, lo, hi):
     """(device address or None, number) of a sampling setting: one number for all rows, or a tensor [rows]."""
-    if torch.is_tensor(value):
-        _require(value.dtype == dtype and value.device == device and value.is_contiguous() and value.numel() == rows,
-                 f"{name} must be a number or a contiguous {dtype} tensor [rows] on the device of the logits")
+    if isinstance(value, torch.Tensor):
+        if value.dtype is not dtype or value.get_device() != index or value.numel() != rows or not value.is_contiguous():
+            raise ValueError(f"{name} must be a number or a contiguous {dtype} tensor [rows] on the device of the logits")
         return value.data_ptr(), 0
-    _require(lo <= value <= hi, f"{name} must lie in [{lo}, {hi}]")
+    if not lo <= value <= hi:
+        raise ValueError(f"{name} must lie in [{lo}, {hi}]")
     return None, value
 
 
@@ -394,22 +408,28 @@ def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     ``check_device_errors``. The sampled counterpart of
     ``dryft/engine/kernels/greedy.py:45-60``."""
     _no_grad(logits)
-    _require(logits.is_cuda and logits.dtype in (BF16, torch.float32) and logits.is_contiguous() and logits.dim() in (1, 2),
-             "expected contiguous bf16 or fp32 CUDA logits [R, V]")
-    dev, vocab = logits.device, logits.shape[-1]
-    rows = 1 if logits.dim() == 1 else logits.shape[0]
-    _require(uniforms.dtype == torch.float32 and uniforms.device == dev and uniforms.is_contiguous()
-             and uniforms.numel() == rows, "uniforms must be a contiguous fp32 tensor [R] on the device of the logits")
-    t, t_all = _setting(temperature, "temperature", rows, torch.float32, dev, 0.0, float("inf"))
-    k, k_all = _setting(top_k, "top_k", rows, torch.int32, dev, 0, 2 ** 31 - 1)
-    p, p_all = _setting(top_p, "top_p", rows, torch.float32, dev, 0.0, 1.0)
-    m, m_all = _setting(min_p, "min_p", rows, torch.float32, dev, 0.0, 1.0)
-    with _on(dev):
-        if out is None:
-            out = torch.empty(rows, dtype=torch.int64, device=dev)
-        _require(out.dtype == torch.int64 and out.device == dev and out.is_contiguous() and out.numel() == rows,
-                 "out must be a contiguous int64 tensor [R] on the device of the logits")
-        _lib.check(_lib.load().qb_sample_token(logits.data_ptr(), int(logits.dtype == torch.float32), rows, vocab,
-                                               uniforms.data_ptr(), t, t_all, k, k_all, p, p_all, m, m_all,
-                                               out.data_ptr(), _status(dev), _raw_stream(dev.index)))
+    index, shape = logits.get_device(), logits.shape
+    fp32 = logits.dtype is torch.float32
+    if index < 0 or not (fp32 or logits.dtype is BF16) or len(shape) not in (1, 2) or not logits.is_contiguous():
+        raise ValueError("expected contiguous bf16 or fp32 CUDA logits [R, V]")
+    vocab = shape[-1]
+    rows = 1 if len(shape) == 1 else shape[0]
+    if (uniforms.dtype is not torch.float32 or uniforms.get_device() != index or uniforms.numel() != rows
+            or not uniforms.is_contiguous()):
+        raise ValueError("uniforms must be a contiguous fp32 tensor [R] on the device of the logits")
+    t, t_all = _setting(temperature, "temperature", rows, torch.float32, index, 0.0, float("inf"))
+    k, k_all = _setting(top_k, "top_k", rows, I32, index, 0, 2 ** 31 - 1)
+    p, p_all = _setting(top_p, "top_p", rows, torch.float32, index, 0.0, 1.0)
+    m, m_all = _setting(min_p, "min_p", rows, torch.float32, index, 0.0, 1.0)
+    if _current_device() != index:
+        with torch.cuda.device(index):
+            return sample_token(logits, uniforms, temperature, top_k, top_p, min_p, out)
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    elif out.dtype is not torch.int64 or out.get_device() != index or out.numel() != rows or not out.is_contiguous():
+        raise ValueError("out must be a contiguous int64 tensor [R] on the device of the logits")
+    rc = _lib.load().qb_sample_token(logits.data_ptr(), fp32, rows, vocab, uniforms.data_ptr(), t, t_all, k, k_all, p,
+                                     p_all, m, m_all, out.data_ptr(), _status(index), _raw_stream(index))
+    if rc:
+        _lib.check(rc)
     return out
