@@ -104,6 +104,76 @@ __device__ __forceinline__ int tile_owner(long long x, long long total, int E) {
 }
 __device__ __forceinline__ long long tile_begin(int i, long long total, int E) { return (long long)i * total / E; }
 
+// Joins the pieces that CTAs cf .. cl left of a unit, in order, and writes its
+// rows: warp w the rows w, w + 4, ..., R of them at once, a lane 4 dims. Bound by
+// the latency of the loads (L2), so 8 / R pieces are loaded at a time.
+template <int R>
+__device__ __forceinline__ void join_pieces(const PagedAttnArgs& a, int warp, int lane, int rows, int cf, int cl,
+                                            int first_slot, int q0, int g) {
+  constexpr int U = 8 / R;
+  auto piece = [&](int c, int i) {
+    return (size_t)(2 * c + (c == cf ? first_slot : 0)) * kPdRows + warp + kPdWarps * i;  // the later ones are their CTAs' first
+  };
+  float top[R], lsum[R];
+  float4 acc[R];
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    top[i] = -INFINITY;
+    lsum[i] = 0.f;
+    acc[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+  }
+  for (int c = cf + lane; c <= cl; c += 32)
+#pragma unroll
+    for (int i = 0; i < R; ++i)
+      if (warp + kPdWarps * i < rows) top[i] = fmaxf(top[i], __ldcg(a.part_ml + piece(c, i) * 2));
+#pragma unroll
+  for (int i = 0; i < R; ++i) top[i] = warp_max(top[i]);
+  for (int c0 = cf; c0 <= cl; c0 += U) {
+    float2 ml[U][R];
+    float4 ov[U][R];
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const bool in = c0 + u <= cl && warp + kPdWarps * i < rows;
+        ml[u][i] = in ? __ldcg(reinterpret_cast<const float2*>(a.part_ml + piece(c0 + u, i) * 2)) : make_float2(-INFINITY, 0.f);
+        ov[u][i] = in ? __ldcg(reinterpret_cast<const float4*>(a.part_o + piece(c0 + u, i) * kAttnD + 4 * lane))
+                      : make_float4(0.f, 0.f, 0.f, 0.f);
+      }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int i = 0; i < R; ++i) {
+        const float w = exp2f(ml[u][i].x - (top[i] == -INFINITY ? 0.f : top[i]));
+        lsum[i] = fmaf(ml[u][i].y, w, lsum[i]);
+        acc[i].x = fmaf(ov[u][i].x, w, acc[i].x);
+        acc[i].y = fmaf(ov[u][i].y, w, acc[i].y);
+        acc[i].z = fmaf(ov[u][i].z, w, acc[i].z);
+        acc[i].w = fmaf(ov[u][i].w, w, acc[i].w);
+      }
+  }
+  const bool has_base = a.sink.base32 != nullptr;
+#pragma unroll
+  for (int i = 0; i < R; ++i) {
+    const int r = warp + kPdWarps * i;
+    if (r >= rows) continue;
+    const size_t row = (size_t)(q0 + r / a.G) * a.Hq + g * a.G + r % a.G;
+    const RowScale rs = row_scale(top[i], lsum[i], has_base, has_base ? a.sink.base_lse[row] : 0.f);
+    float4 v = make_float4(acc[i].x * rs.own, acc[i].y * rs.own, acc[i].z * rs.own, acc[i].w * rs.own);
+    if (has_base) {
+      const float4 bv = *reinterpret_cast<const float4*>(a.sink.base32 + row * kAttnD + 4 * lane);
+      v.x = fmaf(bv.x, rs.other, v.x);
+      v.y = fmaf(bv.y, rs.other, v.y);
+      v.z = fmaf(bv.z, rs.other, v.z);
+      v.w = fmaf(bv.w, rs.other, v.w);
+    }
+    uint2 ob;
+    ob.x = pack_bf16(v.x, v.y);
+    ob.y = pack_bf16(v.z, v.w);
+    *reinterpret_cast<uint2*>(a.sink.out + row * kAttnD + 4 * lane) = ob;
+  }
+}
+
 __host__ inline size_t pd_smem_bytes() {
   return 1024 + (size_t)kPdStages * kPdStageBytes + kPdRows * kPdPStride + 2 * kPdWarps * kPdRows * 4 +
          2 * kPdStages * 8 + 64 + (kPagedMaxSeqs + 1) * 4 + 4 + kPagedMaxSeqs * 8;
@@ -453,44 +523,11 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
         }
         named_barrier(1, kPdWarps * 32);
         if (flag[0]) {
-          // join the pieces of CTAs cf .. cl in order: one row a warp, 4 dims a lane
-          for (int r = warp; r < rows; r += kPdWarps) {
-            auto piece = [&](int c) {
-              return (size_t)(2 * c + (tile_begin(c, total, E) >= u0 ? 0 : 1)) * kPdRows + r;
-            };
-            float top = -INFINITY;
-            for (int c = cf + lane; c <= cl; c += 32) top = fmaxf(top, __ldcg(a.part_ml + piece(c) * 2));
-            top = warp_max(top);
-            const float mu = top == -INFINITY ? 0.f : top;
-            float lsum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-            for (int c = cf; c <= cl; ++c) {
-              const float2 ml = __ldcg(reinterpret_cast<const float2*>(a.part_ml + piece(c) * 2));
-              const float4 ov = __ldcg(reinterpret_cast<const float4*>(a.part_o + piece(c) * kAttnD + 4 * lane));
-              const float w = exp2f(ml.x - mu);
-              lsum = fmaf(ml.y, w, lsum);
-              acc.x = fmaf(ov.x, w, acc.x);
-              acc.y = fmaf(ov.y, w, acc.y);
-              acc.z = fmaf(ov.z, w, acc.z);
-              acc.w = fmaf(ov.w, w, acc.w);
-            }
-            const size_t row = (size_t)(sp.q0 + r / a.G) * a.Hq + g * a.G + r % a.G;
-            const bool has_base = a.sink.base32 != nullptr;
-            const RowScale rs = row_scale(top, lsum, has_base, has_base ? a.sink.base_lse[row] : 0.f);
-            acc.x *= rs.own; acc.y *= rs.own; acc.z *= rs.own; acc.w *= rs.own;
-            if (has_base) {
-              const float4 bv = *reinterpret_cast<const float4*>(a.sink.base32 + row * kAttnD + 4 * lane);
-              acc.x = fmaf(bv.x, rs.other, acc.x);
-              acc.y = fmaf(bv.y, rs.other, acc.y);
-              acc.z = fmaf(bv.z, rs.other, acc.z);
-              acc.w = fmaf(bv.w, rs.other, acc.w);
-            }
-            uint2 ob;
-            ob.x = pack_bf16(acc.x, acc.y);
-            ob.y = pack_bf16(acc.z, acc.w);
-            *reinterpret_cast<uint2*>(a.sink.out + row * kAttnD + 4 * lane) = ob;
-          }
+          const int slot0 = tile_begin(cf, total, E) >= u0 ? 0 : 1;
+          // one, two or four rows a warp at once: eight pieces' loads on their way either way
+          if (rows <= kPdWarps) join_pieces<1>(a, warp, lane, rows, cf, cl, slot0, sp.q0, g);
+          else if (rows <= 2 * kPdWarps) join_pieces<2>(a, warp, lane, rows, cf, cl, slot0, sp.q0, g);
+          else join_pieces<4>(a, warp, lane, rows, cf, cl, slot0, sp.q0, g);
         }
       }
       t += x1 - x0;
