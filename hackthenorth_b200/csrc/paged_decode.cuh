@@ -253,18 +253,18 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
   if (threadIdx.x == 0) pref[0] = 0;
   __syncthreads();
 
-  const long long total = (long long)carry * a.Hkv;
+  const int total = carry * a.Hkv;  // the host keeps the line below 2^31 places
   const int tiles = carry - kPdUnitCost * block_count(live, warp_tot);
-  const int E = (int)min((long long)gridDim.x, max(1ll, (long long)tiles * a.Hkv / kPdMinTiles));
+  const int E = min((int)gridDim.x, max(1, tiles * a.Hkv / kPdMinTiles));
   const int me = blockIdx.x;
   if (me >= E || total == 0) return;
-  const long long t_begin = tile_begin(me, total, E), t_end = tile_begin(me + 1, total, E);
+  const int t_begin = (int)tile_begin(me, total, E), t_end = (int)tile_begin(me + 1, total, E);
   int seq0;  // the sequence of tile t_begin: the last with pref[seq] * Hkv <= t_begin and tiles of its own
   {
     int lo = 0, hi = b.n_seqs - 1;
     while (lo < hi) {
       const int mid = (lo + hi) >> 1;
-      if ((long long)pref[mid + 1] * a.Hkv > t_begin) hi = mid;
+      if (pref[mid + 1] * a.Hkv > t_begin) hi = mid;
       else lo = mid + 1;
     }
     seq0 = lo;
@@ -278,13 +278,13 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
     int issued = 0;
     bool ok = true;
     int seq = seq0;
-    for (long long t = t_begin; t < t_end && ok; ++seq) {
+    for (int t = t_begin; t < t_end && ok; ++seq) {
       const int places = pref[seq + 1] - pref[seq];  // of one head in the line
       if (places == 0) continue;
       const SeqSpan sp = {seqs[seq].x & 0x1ffffff, seqs[seq].x >> 25, seqs[seq].y};
       const TileSpan ts = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks);
-      const long long base = (long long)pref[seq] * a.Hkv;
-      const long long stop = min(t_end, base + (long long)places * a.Hkv);
+      const int base = pref[seq] * a.Hkv;
+      const int stop = min(t_end, base + places * a.Hkv);
       // page of this lane's box of the tile at k, or -1
       auto page_of = [&](int k) {
         const int c0 = (k < ts.n_sink ? k : k - ts.n_sink + ts.lo_tile) * kPdKeys + box * br;
@@ -296,11 +296,11 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
         }
         return page;
       };
-      int k = max(0, (int)((t - base) % places) - kPdUnitCost);
+      int k = max(0, (t - base) % places - kPdUnitCost);
       int page = page_of(k);
       while (t < stop && ok) {
-        const int g = (int)((t - base) / places);
-        const int x0 = (int)(t - base - (long long)g * places), x1 = (int)min((long long)places, x0 + (t_end - t));
+        const int g = (t - base) / places;
+        const int x0 = t - base - g * places, x1 = min(places, x0 + (t_end - t));
         const int k1 = max(0, x1 - kPdUnitCost);
         for (k = max(0, x0 - kPdUnitCost); k < k1; ++k) {
           const int c0 = (k < ts.n_sink ? k : k - ts.n_sink + ts.lo_tile) * kPdKeys + box * br;
@@ -333,22 +333,22 @@ __global__ void __launch_bounds__(kPdThreads, kPdCtasPerSm)
   const float scale = kLog2e * 0.08838834764831845f;  // log2(e) / sqrt(128)
   int used = 0;
   int seq = seq0;
-  for (long long t = t_begin; t < t_end; ++seq) {
+  for (int t = t_begin; t < t_end; ++seq) {
     const int places = pref[seq + 1] - pref[seq], n_tiles = places - kPdUnitCost;
     if (places == 0) continue;
     const SeqSpan sp = {seqs[seq].x & 0x1ffffff, seqs[seq].x >> 25, seqs[seq].y};
     const TileSpan ts = tile_span<kPdKeys>(sp.kv - sp.n, sp.kv, b.window, b.sinks);
-    const long long base = (long long)pref[seq] * a.Hkv;
-    const long long stop = min(t_end, base + (long long)places * a.Hkv);
+    const int base = pref[seq] * a.Hkv;
+    const int stop = min(t_end, base + places * a.Hkv);
     const int rows = sp.n * a.G;
     int pos[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) pos[h] = r_lo + 8 * h < rows ? sp.kv - sp.n + (r_lo + 8 * h) / a.G : -1;
     const int p_first = sp.kv - sp.n;
     while (t < stop) {
-      const int g = (int)((t - base) / places);
-      const long long u0 = base + (long long)g * places;  // the unit's place in the line: first those without a tile
-      const int x0 = (int)(t - u0), x1 = (int)min((long long)places, x0 + (t_end - t));
+      const int g = (t - base) / places;
+      const int u0 = base + g * places;  // the unit's place in the line: first those without a tile
+      const int x0 = t - u0, x1 = min(places, x0 + (t_end - t));
       const int k0 = max(0, x0 - kPdUnitCost), k1 = max(0, x1 - kPdUnitCost);
       if (k0 == k1) {
         t += x1 - x0;

@@ -335,7 +335,8 @@ int qb_grouped_attention_noalloc(const void* q, const void* k_cache, const void*
  *                     of its query rows included; query i of n sits at position
  *                     kv_lens[b] - n + i (a negative one sees nothing: output 0)
  *   tokens            rows of q (and of out)
- * At most 1024 sequences, 64 KV heads and 16 query heads per KV head. Lengths
+ * At most 1024 sequences, 64 KV heads and 16 query heads per KV head, and the
+ * sequences' tables no longer than 2^31 64-key tiles over all KV heads. Lengths
  * and tables are read on the device (a captured graph follows them); numbers
  * outside the call's sizes are reported through device_status (a device int,
  * zero before, for instance the first word of a qb_op_check scratch) and the
@@ -361,7 +362,8 @@ int qb_rope_paged_append(const void* qkv, const void* q_norm, const void* k_norm
 /* Workspace of qb_paged_attention (prefix_tokens 0) and
  * qb_shared_prefix_attention (prefix_tokens: its `tokens`) for calls of up to
  * max_queries; its first qb_paged_zero_bytes() bytes must be zero before its
- * first use (the kernels leave them zero), its address a multiple of 256. Calls
+ * first use (the kernels leave them zero; zero them again after a reported
+ * timeout), its address a multiple of 256. Calls
  * that may overlap on the GPU need a workspace each. */
 size_t qb_paged_zero_bytes(void);
 int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, int prefix_tokens, size_t* bytes);
