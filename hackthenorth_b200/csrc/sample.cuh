@@ -9,24 +9,30 @@
 //   token = the first index at which the running mass of the kept tokens, in
 //   index order, exceeds u times their mass
 //
-// No sort: the last kept rank is found by a histogram. Masses are integers
-// (w 2^44, so a sum of up to 2^18 tokens fits 64 bits), which makes every sum
-// exact and the result independent of the order of the atomics.
+// Masses are integers (w 2^44, so a sum of up to 2^18 tokens fits 64 bits), which
+// makes every sum exact and the result independent of the order of the atomics.
 //
 // A cluster of 8 CTAs holds the row in shared memory, so it is read once.
-// Bound by latency for few rows (a dozen passes over 20 thousand shared-memory
-// values a CTA, each ended by a cluster barrier), by bytes for many.
-//  1. (maximum, its lowest index): the answer of greedy rows (T = 0)
-//  2. tokens counted and weighed in 1024 bins of equal width in (max - x) / T,
-//     1/32 each (the last takes the rest): monotone in x, and unlike bins of
-//     x's own bits not a handful of crowded ones. Each CTA sums its share of the
-//     bins over the cluster and finds whether the border lies there.
-//  3. up to 4096 tokens in the bins up to the border's (nearly always): put in a
-//     list, and one CTA finds the border among them
-//     else: the border's bin again in 1024 sub-bins; a sub-bin whose tokens are not
-//     all equal is split by 8 bits of the value's ordered pattern at a time
-//  4. the kept mass of every warp's stretch of indexes, the stretch that the
-//     target falls in, the token in it
+// Bound by latency: a chain of a few cluster barriers and of code that runs once
+// (one row of 151936: 8 us on the device, 192 rows 150 us, 37 of them at a time,
+// beside 18 us for their bytes). So the work is cut down step by step:
+//  1. the largest token of every lane and warp, and of the row with its lowest
+//     index: the answer of greedy rows (T = 0)
+//  2. what cannot be kept is dropped without being counted: the first top_k
+//     warps' maxima (or as many as hold top-p's mass) are that many tokens, so
+//     nothing below the last of them ranks among the first top_k; where the
+//     warps' 128 are too few, the same with the lanes' 4096, in bins
+//  3. up to 4096 tokens are left: put in a list in index order, and one CTA finds
+//     the border, of up to 256 by counting each one's betters (sorting or a
+//     search by bits took 20 us more), of more by 1024 bins and the border's bin
+//     token by token
+//  4. else (wide nuclei, flat rows): all tokens counted and weighed in 1024 bins
+//     of equal width in (max - x) / T (1/32 each, the last takes the rest:
+//     monotone in x, and unlike bins of x's own bits not a handful of crowded
+//     ones), each CTA summing its share over the cluster; the border's bin again
+//     in 1024 sub-bins, a sub-bin of unequal tokens by 8 bits of their pattern at
+//     a time; then the kept mass of every warp's stretch of indexes, the stretch
+//     that the target falls in, and the token in it (without any filter: this alone)
 #pragma once
 #include "attention.cuh"
 

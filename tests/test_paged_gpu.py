@@ -134,6 +134,8 @@ DECODE = [
     ([(1, 77)], 16, 1, 16),
     ([(3, 50), (2, 333)], 5, 1, 64),
     ([(1, 1 + 37 * i % 400) for i in range(700)], 8, 8, 16),
+    ([(int(i % 3 > 0), 5 + 13 * i % 150) for i in range(1024)], 4, 2, 16),
+    ([(2, 40000)], 16, 2, 64),
 ]
 
 
@@ -205,6 +207,8 @@ PREFIX = [
     ([(9, 30), (40, 300), (1, 2)], 32, 8, 16, 777),
     ([(30, 30)] * 9, 5, 1, 128, 256),
     ([(1, 9), (2, 20)], 16, 8, 16, 0),
+    ([(2, 0), (1, 5), (3, 1)], 16, 8, 16, 40),
+    ([(20, 0), (1, 5)], 16, 8, 16, 300),
 ]
 
 
