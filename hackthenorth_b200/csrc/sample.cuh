@@ -229,7 +229,7 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
   const unsigned top_key = (unsigned)(best >> 32);
   const float top = sample_value(top_key);
 
-  const float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
+  float temperature = a.temperature ? a.temperature[row] : a.temperature_all;
   if (top_key == 0u || !(temperature > 0.f)) {  // nothing to draw, or greedy
     if (rank == 0 && threadIdx.x == 0) {
       if (top_key == 0u) report_error(a.err, DEV_BAD_LOGITS);
@@ -237,16 +237,18 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
     }
     return;  // the same for the whole cluster, and no CTA's memory is read after the barrier
   }
+  if (top == INFINITY) temperature = 1.f;  // an infinite logit takes all the mass at any temperature, infinity too
   const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
   const float top_p = a.top_p ? a.top_p[row] : a.top_p_all;
   const float min_p = fminf(a.min_p ? a.min_p[row] : a.min_p_all, 1.f);
   const float inv_t = fminf(1.f / temperature, 3.402823466e38f);
+  const float mend_below = inv_t > 0.f ? 128.f : 0.f;  // T infinite: the quotient 0 is exact, and T * 0 no number
 
   // (max - x) / T for the bins (0 at the maximum, infinite ones too), and the weight, of the same corrected to a
   // rounding or two of 2^-24: its error would be the weight's.
   auto depth = [&](float x) { return x == top ? 0.f : fminf(top - x, 3.402823466e38f) * inv_t; };
   auto weight = [&](float x, float y) {
-    if (y < 128.f) y = fmaf(fmaf(-y, temperature, x == top ? 0.f : top - x), inv_t, y);
+    if (y < mend_below) y = fmaf(fmaf(-y, temperature, x == top ? 0.f : top - x), inv_t, y);
     return expf(-y);
   };
   auto mass_of = [](float w) { return (unsigned long long)__float2ull_rn(w * kSmOne); };

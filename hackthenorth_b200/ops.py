@@ -404,7 +404,7 @@ def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     of these the ones with at least ``min_p`` of the largest weight; the token
     is the first, by index, at which the kept mass passes ``uniform`` times the
     whole. Temperature 0 takes the largest logit, lowest index on ties, as
-    ``greedy_token``. A row without a finite logit gives -1 and raises in
+    ``greedy_token``; infinity weighs every kept token the same. A row without a finite logit gives -1 and raises in
     ``check_device_errors``. The sampled counterpart of
     ``dryft/engine/kernels/greedy.py:45-60``."""
     _no_grad(logits)
