@@ -241,7 +241,8 @@ __global__ void __cluster_dims__(kSmCluster, 1, 1) __launch_bounds__(kSmThreads,
   const int top_k = a.top_k ? a.top_k[row] : a.top_k_all;
   const float top_p = a.top_p ? a.top_p[row] : a.top_p_all;
   const float min_p = fminf(a.min_p ? a.min_p[row] : a.min_p_all, 1.f);
-  const float inv_t = fminf(1.f / temperature, 3.402823466e38f);
+  temperature = fmaxf(temperature, 1.17549435e-38f);  // 2^-126: below it 1 / T passes fp32
+  const float inv_t = 1.f / temperature;
   const float mend_below = inv_t > 0.f ? 128.f : 0.f;  // T infinite: the quotient 0 is exact, and T * 0 no number
 
   // (max - x) / T for the bins (0 at the maximum, infinite ones too), and the weight, of the same corrected to a

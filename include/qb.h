@@ -403,13 +403,13 @@ int qb_shared_prefix_attention(const void* q, const void* k_pages, const void* v
  * always), min_p > 0 of these the tokens with w_i >= min_p. The token is the
  * first, by index, at which the kept tokens' running mass exceeds uniform times
  * their mass. temperature 0 (or below): the largest logit's lowest index;
- * infinity: every kept token weighs the same. An infinite logit takes all the
- * mass at any temperature, and at a finite one logits further apart than the
- * largest fp32 number count as infinitely far. Each setting is a device array
- * [rows] or, where that is NULL, the value beside it for all rows. Logits of
- * -inf and NaN are never drawn; a row of nothing else gives -1 and is reported.
- * Masses are summed as integers: the result does not depend on the order of
- * execution. */
+ * positive ones below 2^-126 count as 2^-126; infinity: every kept token weighs
+ * the same. An infinite logit takes all the mass at any temperature, and at a
+ * finite one logits further apart than the largest fp32 number count as
+ * infinitely far. Each setting is a device array [rows] or, where that is NULL,
+ * the value beside it for all rows. Logits of -inf and NaN are never drawn; a
+ * row of nothing else gives -1 and is reported. Masses are summed as integers:
+ * the result does not depend on the order of execution. */
 int qb_sample_token(const void* logits, int fp32, int rows, int vocab, const float* uniforms, const float* temperature,
                     float temperature_all, const int* top_k, int top_k_all, const float* top_p, float top_p_all,
                     const float* min_p, float min_p_all, int64_t* token_out, int* device_status, void* stream);

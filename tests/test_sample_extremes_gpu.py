@@ -112,3 +112,17 @@ def test_infinite_logits_take_all_the_mass_at_any_temperature():
         for kw in (dict(), dict(top_k=3), dict(top_p=0.999), dict(top_k=4500, top_p=0.9999)):
             got = ops.sample_token(x, u, t, **kw).tolist()
             assert got == [7] * 32 + [4000] * 32, (t, kw)
+
+
+def test_temperatures_below_the_normal_numbers_count_as_the_least_of_them():
+    from hackthenorth_b200 import ops
+
+    least = 2.0 ** -126
+    u = torch.rand(50, generator=torch.Generator().manual_seed(4)).to(DEV)
+    near = (-torch.arange(300, device=DEV).float() * least).repeat(50, 1)  # weights e^-i at the least temperature
+    far = (-torch.arange(300, device=DEV).float() * 1e-20).repeat(50, 1)
+    for kw in (dict(), dict(top_k=20), dict(top_p=0.9), dict(top_k=280, top_p=0.95)):
+        want = ops.sample_token(near / least, u, 1.0, **kw)
+        for t in (least, 1e-40, 1e-45):
+            assert torch.equal(ops.sample_token(near, u, t, **kw), want), (t, kw)
+            assert bool((ops.sample_token(far, u, t, **kw) == 0).all())
