@@ -194,28 +194,35 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   return r;
 }
 
-// 2^x of two values on the FMA pipe: x = n + f with n the nearest integer, a
-// cubic for 2^f on [-1/2, 1/2] (fitted to the least largest relative error,
-// 2^-13.7, beside P's rounding of 2^-9), n added to the exponent. x is held at
-// -125 or more, so that the result stays a normal number; a NaN becomes the
-// largest finite one.
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two values (below 2^7) on the FMA pipe: x = n + f with n the nearest
+// integer, a cubic for 2^f on [-1/2, 1/2] (fitted to the least largest relative
+// error, 2^-13.7, beside P's rounding of 2^-8), times 2^n from n's bits. The
+// multiplication, unlike an addition to the exponent, keeps a NaN, and gives
+// exactly 0 for x at or below -127, where 2^n's bits are 0: a masked key's V may
+// be 2^128, so any rest of its weight would show.
 __device__ __forceinline__ void exp2_poly(uint64_t x, float& p0, float& p1) {
   constexpr float kC0 = 0.99992807f, kC1 = 0.69326099f, kC2 = 0.24261113f, kC3 = 0.05517167f;
+  constexpr float kRound = 12582912.f + 127.f;  // 1.5 * 2^23, and the exponent's bias: the sum's low bits are n + 127
   float a, b;
   unpack_f32x2(x, a, b);
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-125.f));
-  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-125.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
   x = f32x2(a, b);
-  const uint64_t n = add_f32x2(x, f32x2(12582912.f, 12582912.f));  // 1.5 * 2^23: the sum's low bits are n
-  const uint64_t f = add_f32x2(x, fma_f32x2(n, f32x2(-1.f, -1.f), f32x2(12582912.f, 12582912.f)));
+  const uint64_t n = add_f32x2(x, f32x2(kRound, kRound));
+  const uint64_t f = add_f32x2(x, fma_f32x2(n, f32x2(-1.f, -1.f), f32x2(kRound, kRound)));
   uint64_t p = fma_f32x2(f, f32x2(kC3, kC3), f32x2(kC2, kC2));
   p = fma_f32x2(p, f, f32x2(kC1, kC1));
   p = fma_f32x2(p, f, f32x2(kC0, kC0));
   float n0, n1;
   unpack_f32x2(n, n0, n1);
-  unpack_f32x2(p, p0, p1);
-  p0 = __int_as_float(__float_as_int(p0) + (__float_as_int(n0) << 23));
-  p1 = __int_as_float(__float_as_int(p1) + (__float_as_int(n1) << 23));
+  const float s0 = __int_as_float(__float_as_int(n0) << 23), s1 = __int_as_float(__float_as_int(n1) << 23);
+  unpack_f32x2(mul_f32x2(p, f32x2(s0, s1)), p0, p1);
 }
 
 // A word with its lowest n bits set (n clamped to 0..32).
@@ -732,7 +739,6 @@ __global__ void __launch_bounds__(kPtThreads, 1)
       const bool ok = pv_done(J - 1);
       if (!__all_sync(0xffffffffu, ok)) return false;
       tc_fence_after();
-      if (m_ref == -INFINITY) l = 0.f;  // nothing seen: exp2_poly leaves 2^-125 where the mask is -inf
       const bool whole = un.whole != 0;
       const int slot = 2 * me + (un.first ? 0 : 1);
       const size_t row = (size_t)(un.token0 + token) * a.Hq + un.head * a.G + hj;
