@@ -8,6 +8,8 @@ the CUDA library; there is no PyTorch or CPU fallback.
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import _lib
@@ -179,7 +181,9 @@ def rope_attention(qkv, q_norm, k_norm, cos, sin, keys, values, position, eps=1e
 # These calls run on the device their tensors are on (current or not), on its
 # current stream, and may overlap on different streams: each stream has its own
 # workspace, and a call made while a graph is captured takes one from the
-# graph's own memory, so graphs share none either.
+# graph's own memory, so graphs share none either. Threads may share a stream: a
+# call's launches, which pass their pieces through the workspace, are made under
+# its lock.
 
 I32 = torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (
@@ -201,8 +205,21 @@ def _status(index: int) -> int:
     return buf.data_ptr()
 
 
+class _Workspace:
+    """A stream's memory for paged calls, and the lock under which one call after
+    the other takes it and launches into it (re-entrant: making the memory may
+    run a finalizer that makes a call of its own)."""
+
+    __slots__ = ("lock", "memory", "nbytes", "address")
+
+    def __init__(self):
+        self.lock = threading.RLock()
+        self.memory = None
+        self.nbytes = self.address = 0
+
+
 def _workspace(index: int, stream: int, max_queries: int, hq: int, hkv: int, prefix_tokens: int):
-    """Workspace of a paged call: (the tensor, its size in bytes)."""
+    """(workspace, its size in bytes) of a paged call. Its lock is held: the caller releases it after the launches."""
     key = (index, max_queries, hq, hkv, prefix_tokens)
     nbytes = _workspace_bytes.get(key)
     if nbytes is None:
@@ -211,14 +228,19 @@ def _workspace(index: int, stream: int, max_queries: int, hq: int, hkv: int, pre
         if len(_workspace_bytes) > 4096:
             _workspace_bytes.clear()
         nbytes = _workspace_bytes[key] = n.value
-    captured = _capturing()
-    buf = None if captured else _workspaces.get((index, stream))
-    if buf is None or buf.numel() < nbytes:
-        buf = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-        buf[:8192].zero_()  # qb_paged_zero_bytes()
-        if not captured:
-            _workspaces[index, stream] = buf
-    return buf, nbytes
+    ws = _Workspace() if _capturing() else _workspaces.get((index, stream))
+    if ws is None:
+        ws = _workspaces.setdefault((index, stream), _Workspace())
+    ws.lock.acquire()
+    if ws.nbytes < nbytes:
+        try:
+            memory = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
+            memory[:8192].zero_()  # qb_paged_zero_bytes()
+            ws.memory, ws.nbytes, ws.address = memory, nbytes, memory.data_ptr()
+        except BaseException:
+            ws.lock.release()
+            raise
+    return ws, nbytes
 
 
 def _no_grad(*ts):
@@ -339,12 +361,15 @@ def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0,
         with torch.cuda.device(index):
             return paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window, sinks, max_queries, out)
     out = _rows_out(out, q.shape, q)
-    stream = _raw_stream(index)
+    stream, status = _raw_stream(index), _status(index)
     ws, need = _workspace(index, stream, max_queries, hq, hkv, 0)
-    rc = _lib.load().qb_paged_attention(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
-        q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, max_queries, hq, hkv, window, sinks, out.data_ptr(),
-        ws.data_ptr(), need, _status(index), stream)
+    try:
+        rc = _lib.load().qb_paged_attention(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width,
+            q_start.data_ptr(), kv_lens.data_ptr(), seqs, tokens, max_queries, hq, hkv, window, sinks, out.data_ptr(),
+            ws.address, need, status, stream)
+    finally:
+        ws.lock.release()
     if rc:
         _lib.check(rc)
     return out
@@ -371,12 +396,15 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
             return shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_table, q_start, kv_lens,
                                            max_queries, out)
     out = _rows_out(out, q.shape, q)
-    stream = _raw_stream(index)
+    stream, status = _raw_stream(index), _status(index)
     ws, need = _workspace(index, stream, max_queries, hq, hkv, tokens)
-    rc = _lib.load().qb_shared_prefix_attention(
-        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, prefix_table.data_ptr(),
-        prefix_table.shape[0], prefix_len, page_table.data_ptr(), width, q_start.data_ptr(), kv_lens.data_ptr(), seqs,
-        tokens, max_queries, hq, hkv, out.data_ptr(), ws.data_ptr(), need, _status(index), stream)
+    try:
+        rc = _lib.load().qb_shared_prefix_attention(
+            q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), pages, page, prefix_table.data_ptr(),
+            prefix_table.shape[0], prefix_len, page_table.data_ptr(), width, q_start.data_ptr(), kv_lens.data_ptr(),
+            seqs, tokens, max_queries, hq, hkv, out.data_ptr(), ws.address, need, status, stream)
+    finally:
+        ws.lock.release()
     if rc:
         _lib.check(rc)
     return out

@@ -363,8 +363,10 @@ int qb_rope_paged_append(const void* qkv, const void* q_norm, const void* k_norm
  * qb_shared_prefix_attention (prefix_tokens: its `tokens`) for calls of up to
  * max_queries; its first qb_paged_zero_bytes() bytes must be zero before its
  * first use (the kernels leave them zero; zero them again after a reported
- * timeout), its address a multiple of 256. Calls
- * that may overlap on the GPU need a workspace each. */
+ * timeout), its address a multiple of 256. A call
+ * is up to four launches that hand their pieces on through the workspace: calls
+ * that may overlap on the GPU need a workspace each, and host threads that share
+ * one (and its stream) call one after the other, never two at once. */
 size_t qb_paged_zero_bytes(void);
 int qb_paged_workspace_bytes(int max_queries, int n_heads, int n_kv_heads, int prefix_tokens, size_t* bytes);
 
