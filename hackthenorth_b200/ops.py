@@ -16,6 +16,7 @@ from . import _lib
 
 BF16 = torch.bfloat16
 _scratch = {}
+_scratch_lock = threading.RLock()  # making the memory may run a finalizer that makes a call of its own
 _workspaces = {}
 
 
@@ -26,9 +27,12 @@ def _op_scratch(device) -> torch.Tensor:
     key = torch.device(device).index
     buf = _scratch.get(key)
     if buf is None:
-        n = int(_lib.load().qb_op_scratch_bytes())
-        buf = torch.zeros(n, dtype=torch.uint8, device=device)
-        _scratch[key] = buf
+        with _scratch_lock:  # threads that come here together get the same one
+            buf = _scratch.get(key)
+            if buf is None:
+                n = int(_lib.load().qb_op_scratch_bytes())
+                buf = torch.zeros(n, dtype=torch.uint8, device=device)
+                _scratch[key] = buf
     return buf
 
 
