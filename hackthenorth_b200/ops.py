@@ -32,6 +32,8 @@ def _op_scratch(device) -> torch.Tensor:
             if buf is None:
                 n = int(_lib.load().qb_op_scratch_bytes())
                 buf = torch.zeros(n, dtype=torch.uint8, device=device)
+                if not torch.cuda.is_current_stream_capturing():
+                    torch.cuda.current_stream(device).synchronize()  # zero before a call on another stream uses it
                 _scratch[key] = buf
     return buf
 
