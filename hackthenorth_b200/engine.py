@@ -504,7 +504,7 @@ class Engine:
             shape = (1, len(prompt), max_new_tokens)
             state = self.state
             if (state is None or state.shape != shape or self._bound_state is not state
-                    or getattr(state, "draft_tokens", 0) != k):
+                    or getattr(state, "draft_tokens", 0) != k or state.sampling is not None):
                 state = self.new_state(len(prompt), max_new_tokens, draft_tokens=k)
             ids = torch.tensor(prompt, dtype=torch.int64).pin_memory()
             state.prefill(ids.to(self.device, non_blocking=True))

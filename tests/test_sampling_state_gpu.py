@@ -1,0 +1,25 @@
+"""Sampled decode states: reuse by greedy calls, their own checks, and steps
+taken outside of ``generate``."""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda:0"
+PROMPT = [645, 610, 926, 2984, 3233, 1274, 986, 2860]
+
+
+@pytest.fixture(scope="module")
+def engine(built_lib):
+    from hackthenorth_b200 import Engine
+    from hackthenorth_b200.config import QWEN3_SMALL
+
+    return Engine.from_random(QWEN3_SMALL, seed=0)
+
+
+def test_speculation_does_not_reuse_a_sampled_state(engine):
+    from hackthenorth_b200 import Sampling
+
+    greedy = [s[0] for s in engine.generate([PROMPT], 10, draft_tokens=0)]
+    for seed in range(3):
+        engine.new_state(len(PROMPT), 10, draft_tokens=3, sampling=Sampling(temperature=1e4, seed=seed))
+        assert [s[0] for s in engine.generate([PROMPT], 10, draft_tokens=3)] == greedy
