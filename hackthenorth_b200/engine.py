@@ -136,6 +136,8 @@ class DecodeState:
         # this rank's vocabulary shard under tensor parallelism; [B, V] batched
         vshape = (cfg.vocab // engine.tp_size,) if batch == 1 else (batch, cfg.vocab)
         self.logits = torch.zeros(vshape, dtype=BF16, device=dev) if keep_logits or sampling is not None else None
+        # what drawing reports, for ``check``
+        self._draw_status = torch.zeros(1, dtype=torch.int32, device=dev) if self.logits is not None else None
         self.set_sampling(sampling)
         _lib.check(L.qb_set_batch(engine.ctx, batch), engine.ctx)
         _lib.check(L.qb_bind_state(engine.ctx, self.keys.data_ptr(), self.values.data_ptr(), self.capacity,
@@ -165,7 +167,8 @@ class DecodeState:
 
         s = self.sampling
         self._uniforms.uniform_(generator=self._numbers)
-        ops.sample_token(self.logits, self._uniforms, s.temperature, s.top_k, s.top_p, s.min_p, out=self.token)
+        ops.sample_token(self.logits, self._uniforms, s.temperature, s.top_k, s.top_p, s.min_p, out=self.token,
+                         status=self._draw_status)
 
     # -- the four entry points --------------------------------------------------
     # Prompts of at least this many rows run as dense blocks (tensor-core
@@ -257,7 +260,9 @@ class DecodeState:
 
     def check(self) -> None:
         """Synchronise and raise on a device-side error (bounded wait gave up,
-        token or position out of range)."""
+        token or position out of range, logits without a token to draw)."""
+        if self._draw_status is not None:
+            _lib.check(_lib.load().qb_op_check(self._draw_status.data_ptr(), _lib.stream_handle()))
         _lib.check(_lib.load().qb_check(self.engine.ctx, _lib.stream_handle()), self.engine.ctx)
 
     # -- speculative verification ------------------------------------------------

@@ -427,7 +427,7 @@ def _setting(value, name, rows, dtype, index, lo, hi):
     return None, value
 
 
-def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None):
+def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, out=None, status=None):
     """Draw one token per row: temperature, then top-k, top-p and min-p, from given uniform numbers.
 
     logits ``[R, V]`` (or ``[V]``) bf16 or fp32, V at most 262144; uniforms
@@ -438,8 +438,9 @@ def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     of these the ones with at least ``min_p`` of the largest weight; the token
     is the first, by index, at which the kept mass passes ``uniform`` times the
     whole. Temperature 0 takes the largest logit, lowest index on ties, as
-    ``greedy_token``; infinity weighs every kept token the same. A row without a finite logit gives -1 and raises in
-    ``check_device_errors``. The sampled counterpart of
+    ``greedy_token``; infinity weighs every kept token the same. A row without a logit
+    above -inf gives -1 and raises in ``check_device_errors``, or, with
+    ``status`` (int32 ``[1]``, zero), is reported there. The sampled counterpart of
     ``dryft/engine/kernels/greedy.py:45-60``."""
     _no_grad(logits)
     index, shape = logits.get_device(), logits.shape
@@ -457,13 +458,16 @@ def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
     m, m_all = _setting(min_p, "min_p", rows, torch.float32, index, 0.0, 1.0)
     if _current_device() != index:
         with torch.cuda.device(index):
-            return sample_token(logits, uniforms, temperature, top_k, top_p, min_p, out)
+            return sample_token(logits, uniforms, temperature, top_k, top_p, min_p, out, status)
     if out is None:
         out = torch.empty(rows, dtype=torch.int64, device=logits.device)
     elif out.dtype is not torch.int64 or out.get_device() != index or out.numel() != rows or not out.is_contiguous():
         raise ValueError("out must be a contiguous int64 tensor [R] on the device of the logits")
+    if status is not None and not (_is_i32(status, index) and status.numel() == 1):
+        raise ValueError("status must be an int32 tensor [1] on the device of the logits")
     rc = _lib.load().qb_sample_token(logits.data_ptr(), fp32, rows, vocab, uniforms.data_ptr(), t, t_all, k, k_all, p,
-                                     p_all, m, m_all, out.data_ptr(), _status(index), _raw_stream(index))
+                                     p_all, m, m_all, out.data_ptr(),
+                                     _status(index) if status is None else status.data_ptr(), _raw_stream(index))
     if rc:
         _lib.check(rc)
     return out

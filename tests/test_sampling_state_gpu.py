@@ -23,3 +23,19 @@ def test_speculation_does_not_reuse_a_sampled_state(engine):
     for seed in range(3):
         engine.new_state(len(PROMPT), 10, draft_tokens=3, sampling=Sampling(temperature=1e4, seed=seed))
         assert [s[0] for s in engine.generate([PROMPT], 10, draft_tokens=3)] == greedy
+
+
+@pytest.mark.parametrize("batch", [1, 2])
+def test_check_reports_logits_without_a_token(engine, batch):
+    from hackthenorth_b200 import Sampling, ops
+
+    state = engine.new_state(len(PROMPT), 4, batch=batch, sampling=Sampling())
+    state.prefill(torch.tensor([PROMPT] * batch if batch > 1 else PROMPT, device=DEV))
+    state.check()
+    state.logits.fill_(float("nan"))
+    state._draw()
+    assert state.read_token() == [-1] * batch
+    with pytest.raises(ValueError, match="no token"):
+        state.check()
+    state.check()  # reported once
+    ops.check_device_errors(DEV)  # and not to the operators' callers
