@@ -166,7 +166,8 @@ class DecodeState:
         from . import ops
 
         s = self.sampling
-        self._uniforms.uniform_(generator=self._numbers)
+        with torch.inference_mode():  # the state may have been made in it
+            self._uniforms.uniform_(generator=self._numbers)
         ops.sample_token(self.logits, self._uniforms, s.temperature, s.top_k, s.top_p, s.min_p, out=self.token,
                          status=self._draw_status)
 

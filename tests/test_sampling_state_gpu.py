@@ -39,3 +39,17 @@ def test_check_reports_logits_without_a_token(engine, batch):
         state.check()
     state.check()  # reported once
     ops.check_device_errors(DEV)  # and not to the operators' callers
+
+
+def test_steps_outside_of_generate(engine):
+    """A state that ``generate`` made (in inference mode) takes further steps outside of it."""
+    from hackthenorth_b200 import Sampling
+
+    tokens = list(engine.generate([PROMPT], 3, sampling=Sampling(seed=1)))
+    assert len(tokens) == 3
+    state = engine.new_state(len(PROMPT), 6, sampling=Sampling(seed=1))
+    state.prefill(torch.tensor(PROMPT, device=DEV))
+    with torch.inference_mode():
+        state.set_sampling(Sampling(seed=1))
+    state.step()
+    state.check()
