@@ -11,6 +11,7 @@ from __future__ import annotations
 import threading
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -250,11 +251,16 @@ def _workspace(index: int, stream: int, max_queries: int, hq: int, hkv: int, pre
 
 
 def _no_grad(*ts):
-    """These operators have no backward pass: refuse what would silently lose a gradient."""
+    """These operators have no backward pass and no forward-mode derivative:
+    refuse what would silently lose a gradient or a tangent."""
     if torch.is_grad_enabled():
         for t in ts:
             if t is not None and t.requires_grad:
                 raise ValueError("this operator has no backward pass: use it under torch.no_grad()")
+    if forward_ad._current_level >= 0:
+        for t in ts:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise ValueError("this operator has no forward-mode derivative")
 
 
 def _is_bf16(t, index: int) -> bool:
@@ -310,7 +316,7 @@ def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_tabl
     from ``q_start[B]`` on are left as they are in ``out``. Page ids, lengths
     or positions out of range are skipped and raise in ``check_device_errors``.
     ``dryft/engine/kernels/fused.py:9-30,47-82`` for a ragged batch."""
-    _no_grad(qkv, q_norm, k_norm, k_pages, v_pages)
+    _no_grad(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, out)
     index = qkv.get_device()
     if not (_is_bf16(qkv, index) and _is_bf16(cos, index) and _is_bf16(sin, index)
             and (q_norm is None or _is_bf16(q_norm, index)) and (k_norm is None or _is_bf16(k_norm, index))):
@@ -356,7 +362,7 @@ def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0,
     that is not finite in a key that one row of a sequence sees may reach that
     sequence's other rows. ``dryft/engine/kernels/attention.py:200-237`` for a
     ragged batch."""
-    _no_grad(q, k_pages, v_pages)
+    _no_grad(q, k_pages, v_pages, out)
     index = q.get_device()
     pages, hkv, page, width, seqs = _batch(index, k_pages, v_pages, page_table, q_start, kv_lens)
     tokens, hq, max_queries = _queries(q, hkv, index, max_queries)
@@ -389,7 +395,7 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
     Each query sees the whole prefix and its sequence's own keys up to its
     position; ``kv_lens`` and ``page_table`` count and place the own keys only
     (append them with ``first_position=prefix_len``)."""
-    _no_grad(q, k_pages, v_pages)
+    _no_grad(q, k_pages, v_pages, out)
     index = q.get_device()
     pages, hkv, page, width, seqs = _batch(index, k_pages, v_pages, page_table, q_start, kv_lens)
     tokens, hq, max_queries = _queries(q, hkv, index, max_queries)

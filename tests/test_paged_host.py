@@ -122,3 +122,39 @@ def test_threads_on_one_stream_take_turns(lib):
     for t in threads:
         t.join()
     assert lib.calls == 50 and lib.together == 0
+
+
+def _calls(make, plain):
+    """Every operator with one differentiable argument after the other from ``make``, the others plain."""
+    from hackthenorth_b200 import ops
+
+    append = ["qkv", "q_norm", "k_norm", "cos", "sin", "k_pages", "v_pages", "out"]
+    attend = ["q", "k_pages", "v_pages", "out"]
+    tables = dict(page_table=plain, q_start=plain, kv_lens=plain)
+    for op, names, rest in ((ops.rope_paged_append, append, tables), (ops.paged_attention, attend, tables),
+                            (ops.shared_prefix_attention, attend, dict(tables, prefix_table=plain, prefix_len=0)),
+                            (ops.sample_token, ["logits"], dict(uniforms=plain))):
+        for name in names:
+            yield op, {**{n: plain for n in names}, **rest, name: make}
+
+
+def test_arguments_that_require_a_gradient_are_refused():
+    plain = torch.zeros(2, 3)
+    for op, kw in _calls(torch.zeros(2, 3, requires_grad=True), plain):
+        with pytest.raises(ValueError, match="backward"):
+            op(**kw)
+        with torch.no_grad(), pytest.raises(ValueError, match="expected"):  # on to the next check
+            op(**kw)
+
+
+def test_dual_tensors_are_refused():
+    import torch.autograd.forward_ad as fwd
+
+    plain = torch.zeros(2, 3)
+    with fwd.dual_level():
+        for op, kw in _calls(fwd.make_dual(torch.zeros(2, 3), torch.ones(2, 3)), plain):
+            for grad in (True, False):
+                with torch.set_grad_enabled(grad), pytest.raises(ValueError, match="forward-mode"):
+                    op(**kw)
+        with pytest.raises(ValueError, match="expected"):
+            next(_calls(plain, plain))[0](**next(_calls(plain, plain))[1])
