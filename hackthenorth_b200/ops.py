@@ -282,6 +282,8 @@ def _batch(index: int, k_pages, v_pages, page_table, q_start, kv_lens):
         raise ValueError("page_table, q_start and kv_lens must be contiguous int32 tensors on the device of the queries")
     if len(table) != 2 or len(seqs) != 1 or table[0] != seqs[0] or q_start.shape != (seqs[0] + 1,):
         raise ValueError("expected page_table [B, P], q_start [B + 1], kv_lens [B]")
+    if table[0] >= 1 << 31 or table[1] >= 1 << 31:  # the C call takes 32 bits
+        raise ValueError("at most 1024 sequences, and tables of 2^30 keys")
     return shape[0], shape[1], shape[2], table[1], seqs[0]
 
 
@@ -401,8 +403,8 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
     tokens, hq, max_queries = _queries(q, hkv, index, max_queries)
     if not _is_i32(prefix_table, index) or prefix_table.dim() != 1:
         raise ValueError("prefix_table must be a contiguous int32 tensor [n] on the device of q")
-    if not 0 <= prefix_len <= prefix_table.numel() * page:
-        raise ValueError("prefix_len must lie in 0..prefix_table's keys")
+    if not 0 <= prefix_len <= min(prefix_table.shape[0] * page, 1 << 30) or prefix_table.shape[0] >= 1 << 31:
+        raise ValueError("prefix_len must lie in 0..prefix_table's keys, and not above 2^30")
     if _current_device() != index:
         with torch.cuda.device(index):
             return shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_table, q_start, kv_lens,
@@ -455,6 +457,8 @@ def sample_token(logits, uniforms, temperature=1.0, top_k=0, top_p=1.0, min_p=0.
         raise ValueError("expected contiguous bf16 or fp32 CUDA logits [R, V]")
     vocab = shape[-1]
     rows = 1 if len(shape) == 1 else shape[0]
+    if vocab > 1 << 18 or rows > 1 << 24:  # before the C call's 32 bits
+        raise ValueError("expected at most 2^24 rows of at most 262144 logits")
     if (uniforms.dtype is not torch.float32 or uniforms.get_device() != index or uniforms.numel() != rows
             or not uniforms.is_contiguous()):
         raise ValueError("uniforms must be a contiguous fp32 tensor [R] on the device of the logits")

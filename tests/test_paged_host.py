@@ -158,3 +158,35 @@ def test_dual_tensors_are_refused():
                     op(**kw)
         with pytest.raises(ValueError, match="expected"):
             next(_calls(plain, plain))[0](**next(_calls(plain, plain))[1])
+
+
+@pytest.mark.parametrize("kw", [dict(seqs=(1 << 32) + 2), dict(width=(1 << 32) + 4), dict(seqs=1 << 31)])
+def test_batches_beyond_32_bits_are_refused(lib, kw):
+    """Numbers whose low 32 bits would be a call of another size."""
+    with pytest.raises(ValueError):
+        _attend(**kw)
+    with pytest.raises(ValueError):
+        _attend_prefix(**kw)
+    assert lib.calls == 0
+
+
+@pytest.mark.parametrize("kw", [dict(table=1 << 29, length=(1 << 32) + 5), dict(table=1 << 29, length=1 << 32),
+                                dict(table=(1 << 32) + 5), dict(length=81), dict(length=-1)])
+def test_prefixes_beyond_their_table_or_32_bits_are_refused(lib, kw):
+    with pytest.raises(ValueError):
+        _attend_prefix(**kw)
+    assert lib.calls == 0
+    _attend_prefix(length=80)
+    assert lib.calls == 1
+
+
+@pytest.mark.parametrize("shape", [(1, (1 << 32) + 5), ((1 << 32) + 5,), ((1 << 32) + 1, 1), ((1 << 24) + 1, 8), (2, 262145)])
+def test_logits_beyond_the_limits_are_refused(lib, shape):
+    from hackthenorth_b200 import ops
+
+    rows = shape[0] if len(shape) == 2 else 1
+    with pytest.raises(ValueError):
+        ops.sample_token(OnGpu(*shape), OnGpu(rows, dtype=torch.float32), out=OnGpu(rows, dtype=torch.int64))
+    assert lib.calls == 0
+    ops.sample_token(OnGpu(2, 262144), OnGpu(2, dtype=torch.float32), out=OnGpu(2, dtype=torch.int64))
+    assert lib.calls == 1
