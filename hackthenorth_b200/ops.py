@@ -341,6 +341,8 @@ def rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_tabl
             return rope_paged_append(qkv, q_norm, k_norm, cos, sin, k_pages, v_pages, page_table, q_start, kv_lens, eps,
                                      n_heads, first_position, out)
     out = _rows_out(out, (rows[0], hq, 128), qkv)
+    if seqs == 0:
+        return out  # every row is one of no sequence
     rc = _lib.load().qb_rope_paged_append(
         qkv.data_ptr(), _lib.ptr(q_norm), _lib.ptr(k_norm), cos.data_ptr(), sin.data_ptr(), table[0], eps,
         k_pages.data_ptr(), v_pages.data_ptr(), pages, page, page_table.data_ptr(), width, q_start.data_ptr(),
@@ -375,6 +377,8 @@ def paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window=0,
         with torch.cuda.device(index):
             return paged_attention(q, k_pages, v_pages, page_table, q_start, kv_lens, window, sinks, max_queries, out)
     out = _rows_out(out, q.shape, q)
+    if seqs == 0:
+        return out
     stream, status = _raw_stream(index), _status(index)
     ws, need = _workspace(index, stream, max_queries, hq, hkv, 0)
     try:
@@ -410,6 +414,8 @@ def shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_
             return shared_prefix_attention(q, k_pages, v_pages, prefix_table, prefix_len, page_table, q_start, kv_lens,
                                            max_queries, out)
     out = _rows_out(out, q.shape, q)
+    if seqs == 0:
+        return out
     stream, status = _raw_stream(index), _status(index)
     ws, need = _workspace(index, stream, max_queries, hq, hkv, tokens)
     try:

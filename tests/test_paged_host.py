@@ -190,3 +190,15 @@ def test_logits_beyond_the_limits_are_refused(lib, shape):
     assert lib.calls == 0
     ops.sample_token(OnGpu(2, 262144), OnGpu(2, dtype=torch.float32), out=OnGpu(2, dtype=torch.int64))
     assert lib.calls == 1
+
+
+def test_a_batch_of_no_sequences_leaves_every_row(lib):
+    from hackthenorth_b200 import ops
+
+    for tokens in (0, 3):
+        batch, q = _batch(seqs=0, tokens=tokens)
+        assert ops.paged_attention(q, **batch, out=q) is q
+        assert ops.shared_prefix_attention(q, prefix_table=OnGpu(5, dtype=I32), prefix_len=70, **batch, out=q) is q
+        cos = OnGpu(64, 128)
+        assert ops.rope_paged_append(OnGpu(tokens, 8 * 128), None, None, cos, cos, **batch, out=q) is q
+    assert lib.calls == 0
