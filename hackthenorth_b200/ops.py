@@ -242,7 +242,7 @@ def _workspace(index: int, stream: int, max_queries: int, hq: int, hkv: int, pre
     if ws.nbytes < nbytes:
         try:
             memory = torch.empty(nbytes, dtype=torch.uint8, device=torch.device("cuda", index))
-            memory[:8192].zero_()  # qb_paged_zero_bytes()
+            memory[:_lib.load().qb_paged_zero_bytes()].zero_()
             ws.memory, ws.nbytes, ws.address = memory, nbytes, memory.data_ptr()
         except BaseException:
             ws.lock.release()
