@@ -28,9 +28,10 @@
 //  * warps 4-7 and 8-11: softmax of M tile 0 and 1, a thread per row. The
 //    reference maximum only moves when a row's maximum grows by more than 8 (P
 //    stays below 2^8 and keeps its relative precision), so O is seldom rescaled.
-//    Both groups tend to reach their exponentials together; a third of them on
-//    the FMA pipe (a cubic of 13.7 bits) saved 4 of 575 us, and its error went
-//    into the row sums: every one is the MUFU's.
+//    Both groups tend to reach their exponentials together, so every fourth
+//    pair is computed on the FMA pipe, to the MUFU's precision: 548 us for the
+//    8100 tokens against 568 without it, 556 and 552 with every third and fifth
+//    pair; at the power cap 580 either way.
 //  * warp 2: walks the CTA's pieces of units ahead of the others and hands them
 //    over through a ring of 4 (the lookups and divisions of a new piece took 3 us
 //    of every role's time when each made them itself); and waits for K and V on
@@ -55,6 +56,7 @@ constexpr int kPtMinTiles = 2;
 constexpr int kPtUnitCost = 4;  // what beginning and ending a unit takes, in key tiles: its place in the line
 
 constexpr int kPtPieces = 4;
+constexpr int kPtPolyEvery = 4;  // every fourth pair of P comes from exp2_poly, the rest from the MUFU
 
 // What a CTA does next: the key tiles [k0, k1) of a unit (a role's whole state).
 struct PtPiece {
@@ -191,6 +193,39 @@ __device__ __forceinline__ uint64_t add_f32x2(uint64_t a, uint64_t b) {
   uint64_t r;
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
   return r;
+}
+
+__device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+
+// 2^x of two values (below 2^7) on the FMA pipe: x = n + f with n the nearest
+// integer, 2^f on [-1/2, 1/2] by 1 + f q(f) with a quartic q (fitted to the least
+// largest relative error: 2^-22.5 as evaluated in fp32, and none at whole x),
+// times 2^n from n's bits. The multiplication, unlike an addition to the
+// exponent, keeps a NaN, and gives exactly 0 for x at or below -127, where 2^n's
+// bits are 0: a masked key's V may be 2^128, so any rest of its weight would show.
+__device__ __forceinline__ void exp2_poly(uint64_t x, float& p0, float& p1) {
+  constexpr float kC1 = 0.69314700f, kC2 = 0.24022242f, kC3 = 0.055507336f, kC4 = 0.0096715130f, kC5 = 0.0013264727f;
+  constexpr float kRound = 12582912.f + 127.f;  // 1.5 * 2^23, and the exponent's bias: the sum's low bits are n + 127
+  float a, b;
+  unpack_f32x2(x, a, b);
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(a) : "f"(-127.f));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(b) : "f"(-127.f));
+  x = f32x2(a, b);
+  const uint64_t n = add_f32x2(x, f32x2(kRound, kRound));
+  const uint64_t f = add_f32x2(x, fma_f32x2(n, f32x2(-1.f, -1.f), f32x2(kRound, kRound)));
+  uint64_t p = fma_f32x2(f, f32x2(kC5, kC5), f32x2(kC4, kC4));
+  p = fma_f32x2(p, f, f32x2(kC3, kC3));
+  p = fma_f32x2(p, f, f32x2(kC2, kC2));
+  p = fma_f32x2(p, f, f32x2(kC1, kC1));
+  p = fma_f32x2(p, f, f32x2(1.f, 1.f));
+  float n0, n1;
+  unpack_f32x2(n, n0, n1);
+  const float s0 = __int_as_float(__float_as_int(n0) << 23), s1 = __int_as_float(__float_as_int(n1) << 23);
+  unpack_f32x2(mul_f32x2(p, f32x2(s0, s1)), p0, p1);
 }
 
 // A word with its lowest n bits set (n clamped to 0..32).
@@ -684,9 +719,13 @@ __global__ void __launch_bounds__(kPtThreads, 1)
         for (int c = 0; c < 64; c += 2) {
           const uint64_t x = fma_f32x2(f32x2(__uint_as_float(sr[c]), __uint_as_float(sr[c + 1])), scale2, mu2);
           float p0, p1;
-          unpack_f32x2(x, p0, p1);
-          p0 = ex2_approx(p0);
-          p1 = ex2_approx(p1);
+          if ((c >> 1) % kPtPolyEvery == kPtPolyEvery - 1) {
+            exp2_poly(x, p0, p1);
+          } else {
+            unpack_f32x2(x, p0, p1);
+            p0 = ex2_approx(p0);
+            p1 = ex2_approx(p1);
+          }
           rs[(c >> 1) & 1] = add_f32x2(rs[(c >> 1) & 1], f32x2(p0, p1));
           sr[c >> 1] = pack_bf16(p0, p1);
         }
