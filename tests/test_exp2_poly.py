@@ -14,7 +14,7 @@ def test_polynomial_is_as_exact_as_its_comment_says():
     text = open(SOURCE).read()
     coefficients = [np.float32(1)] + [np.float32(re.search(rf"kC{i} = ([0-9.]+)f", text).group(1)) for i in range(1, 6)]
     f32 = lambda x: x.astype(np.float32)
-    x = f32(np.linspace(-127, 8, 2000001))
+    x = f32(np.concatenate((np.linspace(-127, 8, 2000001), np.arange(-127, 9))))
     bias = np.float32(12582912.0 + 127.0)  # as kRound
     n = f32(x + bias)
     f = f32(x + f32(bias - n))
