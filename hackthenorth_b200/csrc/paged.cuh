@@ -156,7 +156,7 @@ __global__ void __launch_bounds__(kAppThreads) paged_append_kernel(const AppendA
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, d);
         if (turn && gain != nullptr) {
-          const float inv = rsqrtf(ss * (1.0f / kAttnD) + a.eps);  // within 2^-22; the one rounding at the end is 2^-9
+          const float inv = rsqrtf(ss * (1.0f / kAttnD) + a.eps);  // within 2^-22; the one rounding at the end is 2^-8
           const uint4 gv = ld128(gain + 8 * j);
           const uint32_t g2[4] = {gv.x, gv.y, gv.z, gv.w};
 #pragma unroll

@@ -5,10 +5,11 @@
 // The formula and the masks are those of paged_decode.cuh. A unit is up to 256
 // query rows of one sequence (two M = 128 tiles of 128 / G tokens with the G
 // query heads of one KV head) against the 64-key tiles that some of its rows
-// sees. As there, the units' tiles form one line which is cut evenly over the
+// see. As there, the units' tiles form one line which is cut evenly over the
 // CTAs (one per SM), a unit's own start and end counted as four tiles (without
-// that the CTAs with many short units of a causal prompt finished last: 716 us
-// for 8100 tokens of 32/8 heads, 508 us with it, 516 us with seven tiles). A cut
+// that the CTAs with many short units of a causal prompt finished last: 746 us
+// for 8100 tokens of 32/8 heads at the power cap, 618 with two tiles, 582 with
+// four, 588 with seven). A cut
 // unit leaves (m, l, O) of its pieces in the workspace, and paged_join_kernel
 // joins them: with 256 rows a piece is 128 KB, too much for one CTA to join
 // behind the others.
@@ -16,7 +17,8 @@
 // Bound, where every key tile meets 256 rows, by the softmax and the MMAs
 // together (about 2000 cycles a key tile; the MMAs alone take 1280: 384 for S,
 // whose operands come from shared memory, and 256 for P.V of each M tile), and
-// by the cache's bytes below that. 8100 prompt tokens: 1.06 PFLOP/s.
+// by the cache's bytes below that. 8100 prompt tokens: 545 us (0.99 PFLOP/s) with
+// pauses between the calls, 578 (0.93) call after call, at the power cap.
 //  * warp 0: TMA. Q tiles (3D map, 128-byte swizzle) and K and V tiles of
 //    16 KB, a box per page, into four slots each.
 //  * warps 1 and 3: the MMAs of M tile 0 and 1. S_t = Q_t . K^T goes to one of
@@ -29,9 +31,9 @@
 //    reference maximum only moves when a row's maximum grows by more than 8 (P
 //    stays below 2^8 and keeps its relative precision), so O is seldom rescaled.
 //    Both groups tend to reach their exponentials together, so every fourth
-//    pair is computed on the FMA pipe, to the MUFU's precision: 548 us for the
+//    pair is computed on the FMA pipe, to the MUFU's precision: 545 us for the
 //    8100 tokens against 568 without it, 556 and 552 with every third and fifth
-//    pair; at the power cap 580 either way.
+//    pair; at the power cap 578 to 581 without, with every fourth and fifth.
 //  * warp 2: walks the CTA's pieces of units ahead of the others and hands them
 //    over through a ring of 4 (the lookups and divisions of a new piece took 3 us
 //    of every role's time when each made them itself); and waits for K and V on

@@ -53,7 +53,8 @@ def _bf16_cuda(*ts):
 
 
 def check_device_errors(device=None) -> None:
-    """Synchronise and raise if an op-level kernel reported a device error."""
+    """Synchronise with the current stream and raise if an op-level kernel reported
+    a device error (calls on other streams report once they have run)."""
     device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
     with torch.cuda.device(device):
         buf = _op_scratch(torch.device("cuda", torch.cuda.current_device()))
@@ -190,7 +191,9 @@ def rope_attention(qkv, q_norm, k_norm, cos, sin, keys, values, position, eps=1e
 # workspace, and a call made while a graph is captured takes one from the
 # graph's own memory, so graphs share none either. Threads may share a stream: a
 # call's launches, which pass their pieces through the workspace, are made under
-# its lock.
+# its lock. A stream's workspace is kept at the largest size it was asked for (39 MB
+# above 16 query rows per KV head, and 512 bytes a row and head with a prefix).
+# ``out`` must not overlap an input.
 
 I32 = torch.int32
 _raw_stream = torch._C._cuda_getCurrentRawStream if hasattr(torch._C, "_cuda_getCurrentRawStream") else (

@@ -335,8 +335,10 @@ int qb_grouped_attention_noalloc(const void* q, const void* k_cache, const void*
  *                     of its query rows included; query i of n sits at position
  *                     kv_lens[b] - n + i (a negative one sees nothing: output 0)
  *   tokens            rows of q (and of out)
- * At most 1024 sequences, 64 KV heads and 16 query heads per KV head, and the
- * sequences' tables no longer than 2^31 64-key tiles over all KV heads. Lengths
+ * At most 1024 sequences, 64 KV heads and 16 query heads per KV head, 4096
+ * blocks of 2 (128 / group) query rows (a new one for each sequence), and the
+ * sequences' tables no longer than 2^31 64-key tiles over all KV heads. Outputs
+ * must not overlap inputs. Lengths
  * and tables are read on the device (a captured graph follows them); numbers
  * outside the call's sizes are reported through device_status (a device int,
  * zero before, for instance the first word of a qb_op_check scratch) and the
