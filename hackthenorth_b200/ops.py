@@ -260,7 +260,7 @@ def _no_grad(*ts):
         for t in ts:
             if t is not None and t.requires_grad:
                 raise ValueError("this operator has no backward pass: use it under torch.no_grad()")
-    if forward_ad._current_level >= 0:
+    if getattr(forward_ad, "_current_level", -1) >= 0:
         for t in ts:
             if t is not None and forward_ad.unpack_dual(t).tangent is not None:
                 raise ValueError("this operator has no forward-mode derivative")
