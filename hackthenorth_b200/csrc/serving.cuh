@@ -58,10 +58,10 @@ int tc_grid() { return std::min(current_sm_count(), kPagedMaxTcCtas); }
 
 // Whether the few-rows kernel takes the call: its 16 MMA rows hold every
 // sequence's query rows of a KV head. Measured against the other one (32/8
-// heads, pages of 64, 4 and 16 rows a head): one sequence of 1000 keys 10.7 and
-// 14.8 against 16.3 us, of 32768 keys 33 and 43 against 43 us, 32 of 4096 keys
-// 91 and 95 against 115 us, 64 of 500 keys 33 and 37 against 52 us. Above 16
-// rows it would read the cache twice.
+// heads, pages of 64, 4 and 16 rows a head, captured): one sequence of 1000
+// keys 10 and 14 against 16 us, of 32768 keys 32 and 40 against 43 us, of 131072
+// keys 91 and 99 against 113 us, 32 of 4096 keys 90 and 92 against 120 us, 64 of
+// 500 keys 31 and 35 against 51 us. Above 16 rows it would read the cache twice.
 bool few_rows(int max_queries, int G) { return (long long)max_queries * G <= kPdRows; }
 
 PagedWorkspace workspace_for(int max_queries, int G, int n_heads, int prefix_tokens) {
